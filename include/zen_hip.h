@@ -63,6 +63,7 @@ extern "C" {
 
 #define ZEN_F32 0
 #define ZEN_BF16 1
+#define ZEN_F16 2 /* what follows "update behind the exchange" only */
 
 /* host return codes */
 #define ZEN_OK 0
@@ -684,6 +685,92 @@ int zen_profile_every(int n);
 int zen_profile_tags(void);
 const char *zen_profile_name(int tag);
 int zen_profile_read(int tag, double *total_ms, int64_t *launches);
+
+/* ------------------------------------------------- update behind the exchange */
+
+/*
+ * Momentum and update of an optimiser step, from the gradient g as the hook returns it (dense, `grad` not null):
+ *   momentum' = mu * momentum + g;   update = nesterov ? g + mu * momentum' : momentum'
+ * in fp32, each output rounded once.  momentum (ZEN_F32 or ZEN_BF16) is updated in place; grad and update are ZEN_F32,
+ * ZEN_BF16 or ZEN_F16.  update may be grad itself if the types are the same, else no two of them may overlap.
+ */
+int zen_momentum(void *momentum, int momentum_dtype, const void *grad, int grad_dtype, int64_t n, float mu, int nesterov,
+                 void *update, int update_dtype, void *stream);
+
+/*
+ * The same where g is the sum of `lists` ascending (index, value) lists, as zen_merge or the second exchange leave them:
+ * idx / val / lengths are HOST arrays of `lists` entries (1 .. ZEN_MOMENTUM_LISTS_MOST) with device addresses and element
+ * counts; counts (null: none) is a HOST array of device addresses of int64 counts (or null), of which the smaller of
+ * count and length holds.  All lists have one index type (idx64) and one value type.  n < 2^31.  Every index once to a list; an
+ * index that several lists hold gets their values in the order of the lists.  An index outside [0, n), or one that is not larger than
+ * its list's last one, sets ZEN_STAT_BAD_INDEX; then neither momentum nor update is written.
+ */
+#define ZEN_MOMENTUM_LISTS_MOST 64
+size_t zen_momentum_lists_workspace(int64_t n, int lists);
+int zen_momentum_lists(void *momentum, int momentum_dtype, const void *const *idx, int idx64, const void *const *val,
+                       int val_dtype, const int64_t *lengths, const int64_t *const *counts, int lists, int64_t n, float mu,
+                       int nesterov, void *update, int update_dtype, void *workspace, size_t workspace_bytes,
+                       int32_t *status, void *stream);
+
+/*
+ * out = alpha * a b + beta * c, a (m x k) and b (k x n) ZEN_BF16 or ZEN_F16, sums in fp32, out rounded once.  Strides count
+ * elements: x_rs from row to row, x_cs from column to column, x_batch from matrix to matrix.  a and b in whatever strides:
+ * where one of the two is 1 and addresses and the other stride are multiples of 16 bytes (for b with b_rs == 1, and a with
+ * a_cs == 1, k too), they are read as they lie, else they are laid out in the workspace first.  c (null: none) and out: any
+ * strides, ZEN_F32, ZEN_BF16 or ZEN_F16; out may be c itself (the same addresses and strides), else it overlaps nothing.
+ * symmetric: the caller vouches that a b is (m == n): half of it is computed and mirrored.
+ */
+typedef struct zen_product_args {
+  const void *a;
+  int64_t a_rs, a_cs, a_batch;
+  const void *b;
+  int64_t b_rs, b_cs, b_batch;
+  int dtype;
+  const void *c;
+  int c_dtype;
+  int64_t c_rs, c_cs, c_batch;
+  void *out;
+  int out_dtype;
+  int64_t out_rs, out_cs, out_batch;
+  int64_t m, n, k, batch;
+  float alpha, beta;
+  int symmetric;
+  void *workspace;
+  size_t workspace_bytes;
+  void *stream;
+} zen_product_args;
+size_t zen_product_workspace(const zen_product_args *args); /* 0: none is needed */
+int zen_product(const zen_product_args *args);
+
+/*
+ * Orthogonalisation of updates (rows x cols, `count` of them, one type and one pair of strides) by Newton-Schulz steps:
+ *   X = U / (|U|_F + eps);   `steps` times  X = a X + (b A + c A A) X  with A = X X^T (X with rows <= cols: turned if need be)
+ * and out = X (weights null), or, applied to weights in place,  W = keep * W - gain * X.
+ * updates, outs and weights are HOST arrays of device addresses.  Types: any of the three for each.  `precise`: every operand is
+ * held in 22 bits (two of fp16) and a product is three (results to fp32's accuracy); else the operands of the
+ * products are fp16 and X is carried from step to step in 22 bits.
+ * An update of zeros gives zeros.  outs may be the updates themselves (same type and strides), else nothing overlaps.
+ */
+typedef struct zen_orthogonal_args {
+  const void *const *updates;
+  int update_dtype;
+  int64_t update_rs, update_cs;
+  void *const *outs; /* or the weights */
+  int out_dtype;
+  int64_t out_rs, out_cs;
+  int64_t rows, cols, count;
+  int steps;
+  float a, b, c;
+  double eps;
+  int precise;
+  int weights; /* outs are weights: W = keep * W - gain * X */
+  float keep, gain;
+  void *workspace;
+  size_t workspace_bytes;
+  void *stream;
+} zen_orthogonal_args;
+size_t zen_orthogonal_workspace(int64_t rows, int64_t cols, int64_t count, int precise);
+int zen_orthogonal(const zen_orthogonal_args *args);
 
 #ifdef __cplusplus
 }

@@ -7,3 +7,5 @@ from .tensor_load_balance import TensorPartition  # noqa: F401
 from .comm import LoadBalanceAllreduce, LocalGroup  # noqa: F401
 from .compress import compress, compress_with_allgather, topk_threshold  # noqa: F401
 from .hook import SparseCommHook  # noqa: F401
+from .update import momentum_update, momentum_update_sparse, orthogonal_step, orthogonalize, product  # noqa: F401
+from .muon import Muon  # noqa: F401

@@ -26,7 +26,7 @@ try:
 except ImportError as e:  # not built, or for another torch
     host = _Unbuilt(str(e))
 
-F32, BF16 = 0, 1
+F32, BF16, F16 = 0, 1, 2  # F16: the operators of update.py only
 OK, EINVAL, EHIP, EWORKSPACE = 0, -1, -2, -3
 STAT_SERIAL_OVERFLOW, STAT_CAPACITY, STAT_INTERNAL, STAT_BAD_INDEX, STAT_RETRY = 1, 2, 4, 8, 16
 MODE_FAST, MODE_GENERAL = 0, 1
@@ -43,6 +43,7 @@ LIB_PATH = os.environ.get("ZEN_HIP_LIB") or os.path.join(_HERE, "csrc", "libzen_
 
 # ZEN_ABI_VERSION of include/zen_hip.h this loader's signatures and structs are written for
 ABI_VERSION = 11
+MOMENTUM_LISTS_MOST = 64  # ZEN_MOMENTUM_LISTS_MOST
 TABLE_SIZES_MOST = 1024  # ZEN_TABLE_SIZES_MOST
 
 _lib = None
@@ -63,6 +64,33 @@ class EncodeMergeArgs(ctypes.Structure):
         ("stream", _vp), ("merge_stream", _vp),
         ("next_input", _vp), ("next_k", _i64), ("next_n", _i64), ("next_m", _i64), ("next_capacity", _i64),
         ("next_table", _vp),
+    ]
+
+
+class ProductArgs(ctypes.Structure):
+    """zen_product_args of include/zen_hip.h."""
+    _vp, _i32, _i64, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
+    _fields_ = [
+        ("a", _vp), ("a_rs", _i64), ("a_cs", _i64), ("a_batch", _i64),
+        ("b", _vp), ("b_rs", _i64), ("b_cs", _i64), ("b_batch", _i64), ("dtype", _i32),
+        ("c", _vp), ("c_dtype", _i32), ("c_rs", _i64), ("c_cs", _i64), ("c_batch", _i64),
+        ("out", _vp), ("out_dtype", _i32), ("out_rs", _i64), ("out_cs", _i64), ("out_batch", _i64),
+        ("m", _i64), ("n", _i64), ("k", _i64), ("batch", _i64),
+        ("alpha", ctypes.c_float), ("beta", ctypes.c_float), ("symmetric", _i32),
+        ("workspace", _vp), ("workspace_bytes", _sz), ("stream", _vp),
+    ]
+
+
+class OrthogonalArgs(ctypes.Structure):
+    """zen_orthogonal_args of include/zen_hip.h."""
+    _vp, _i32, _i64, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
+    _f32 = ctypes.c_float
+    _fields_ = [
+        ("updates", ctypes.POINTER(_vp)), ("update_dtype", _i32), ("update_rs", _i64), ("update_cs", _i64),
+        ("outs", ctypes.POINTER(_vp)), ("out_dtype", _i32), ("out_rs", _i64), ("out_cs", _i64),
+        ("rows", _i64), ("cols", _i64), ("count", _i64), ("steps", _i32), ("a", _f32), ("b", _f32), ("c", _f32),
+        ("eps", ctypes.c_double), ("precise", _i32), ("weights", _i32), ("keep", _f32), ("gain", _f32),
+        ("workspace", _vp), ("workspace_bytes", _sz), ("stream", _vp),
     ]
 
 
@@ -153,6 +181,14 @@ def lib():
         "zen_table_find": (i32, [vp, i64, i32, i64, vp, vp, sz, vp, vp]),
         "zen_table_find_sizes": (i32, [vp, i64, i32, i64, vp, vp, vp, sz, vp, vp, i64, vp]),
         "zen_table_gather": (i32, [vp, i64, i32, vp, i32, i64, vp, vp, i64, vp, sz, vp]),
+        "zen_momentum": (i32, [vp, i32, vp, i32, i64, ctypes.c_float, i32, vp, i32, vp]),
+        "zen_momentum_lists_workspace": (sz, [i64, i32]),
+        "zen_momentum_lists": (i32, [vp, i32, ctypes.POINTER(vp), i32, ctypes.POINTER(vp), i32, ctypes.POINTER(i64),
+                                     ctypes.POINTER(vp), i32, i64, ctypes.c_float, i32, vp, i32, vp, sz, vp, vp]),
+        "zen_product_workspace": (sz, [ctypes.POINTER(ProductArgs)]),
+        "zen_product": (i32, [ctypes.POINTER(ProductArgs)]),
+        "zen_orthogonal_workspace": (sz, [i64, i64, i64, i32]),
+        "zen_orthogonal": (i32, [ctypes.POINTER(OrthogonalArgs)]),
         "zen_stream_read": (i32, [vp, sz, vp, vp]),
         "zen_profile_enable": (i32, [i32]),
         "zen_profile_only": (i32, [i32]),

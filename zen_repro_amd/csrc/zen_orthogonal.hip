@@ -1,0 +1,238 @@
+// Updates made orthogonal by Newton-Schulz steps:  X <- a X + (b A + c A A) X,  A = X X^T,  from X = U / (|U| + eps).
+//
+// A step is three products (zen_tiles.h).  A and A A are symmetric: the tiles of the lower triangle are computed and
+// mirrored.  X is kept with rows <= columns (a tall update is turned when it is laid out, its result when it goes out).
+// Bound by the matrix instructions: 3 m m n + m m m flops a step.
+//
+// Everything is held as fp16 times kUnit, with kUnit = 2^10: a value of 1 is far from fp16's limits and what rounding leaves over
+// is far from its denormals.  Why fp16 and not bf16: entries stay below 2, so range is not needed, and the iteration
+// amplifies rounding (errors against 64 bits, Gaussian update 1024 x 1024: bf16 2e-2, fp16 1e-3).  Where a direction starts
+// small it grows by `a` a step, and so does the noise that rounding X adds to it; so X is carried on as two fp16 (22 bits) and
+// only the products see 11 of them.  The last two steps are written as X + (b A + c A A + (a - 1) I) X: there
+// the singular values are near 1, the bracket is near zero, and so is what rounding it does.  With `precise` the
+// products see 22 bits of every operand too: A B + A B' + A' B, what is left out is below 2^-22.
+#include "zen_tiles.h"
+
+namespace zen {
+namespace {
+
+constexpr float kUnit = 1024.f;
+constexpr int kSquareBlock = 256;
+constexpr int kMostShares = 256;  // workgroups to a matrix' sum of squares
+
+using Tile = TileShape<128, 128, 2, 2>;
+constexpr int kSide = 128;
+
+// Sums of squares in fp64 (an fp32 square overflows from 2^64 on), one a workgroup, in a fixed order.
+__global__ __launch_bounds__(kSquareBlock) void k_squares(MatList in, int64_t rs, int64_t cs, int dtype, int rows, int cols,
+                                                          int shares, double *__restrict__ sums) {
+  __shared__ double s_sum[kSquareBlock / 64];
+  const int share = blockIdx.x, z = blockIdx.y;
+  const char *p = in.of(z);
+  const int64_t slow = cs <= rs ? rows : cols, fast = cs <= rs ? cols : rows;
+  const int64_t slow_stride = cs <= rs ? rs : cs, fast_stride = cs <= rs ? cs : rs;
+  double sum = 0.0;
+  for (int64_t i = share; i < slow; i += shares)
+    for (int64_t j = threadIdx.x; j < fast; j += kSquareBlock) {
+      const double v = (double)load_value(p, i * slow_stride + j * fast_stride, dtype);
+      sum = fma(v, v, sum);
+    }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+  if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double all = 0.0;
+    for (int w = 0; w < kSquareBlock / 64; ++w) all += s_sum[w];
+    sums[(int64_t)z * shares + share] = all;
+  }
+}
+
+// A chunk's buffers: `batch` matrices at once.
+struct Room {
+  int64_t m, n;  // rows and columns, whole tiles
+  int batch;
+  _Float16 *x[2], *x_low[2];  // X takes turns; without `precise` its low half is updated in place
+  _Float16 *a, *a_low, *b, *b_low;
+  double *squares;
+  size_t bytes;
+};
+
+int shares_of(int64_t rows, int64_t cols) {
+  const int64_t want = rows * cols / 8192 + 1, slow = rows > cols ? rows : cols;
+  const int64_t most = want < kMostShares ? want : kMostShares;
+  return (int)(most < slow ? most : slow);
+}
+
+int chunk_of(int64_t m, int64_t n, int64_t count) {
+  // enough matrices at once to fill the card, no more room than some 2 GiB where one matrix does
+  int64_t most = (1ll << 28) / (m * n);
+  if (most < 1) most = 1;
+  if (most > kMostList) most = kMostList;
+  return (int)(count < most ? count : most);
+}
+
+Room room_for(int64_t rows, int64_t cols, int64_t count, bool precise, void *at) {
+  Room r = {};
+  const int64_t small = rows < cols ? rows : cols, large = rows < cols ? cols : rows;
+  r.m = ceil_div(small, kSide) * kSide;
+  r.n = ceil_div(large, kSide) * kSide;
+  r.batch = chunk_of(r.m, r.n, count);
+  Carver cv(at);
+  const size_t xs = (size_t)r.batch * r.m * r.n, as = (size_t)r.batch * r.m * r.m;
+  r.x[0] = cv.take<_Float16>(xs);
+  r.x[1] = cv.take<_Float16>(xs);
+  r.x_low[0] = cv.take<_Float16>(xs);
+  r.x_low[1] = precise ? cv.take<_Float16>(xs) : r.x_low[0];
+  r.a = cv.take<_Float16>(as);
+  r.b = cv.take<_Float16>(as);
+  if (precise) {
+    r.a_low = cv.take<_Float16>(as);
+    r.b_low = cv.take<_Float16>(as);
+  }
+  r.squares = cv.take<double>((size_t)r.batch * shares_of(rows, cols));
+  r.bytes = cv.used;
+  return r;
+}
+
+MatOperand operand(const _Float16 *p, const _Float16 *low, int64_t ld, int64_t batch) {
+  return {{reinterpret_cast<const uint16_t *>(p), reinterpret_cast<const uint16_t *>(low)}, ld, batch};
+}
+
+int chunk(const zen_orthogonal_args &p, const Room &r, int64_t first, int batch, hipStream_t s) {
+  const bool turn = p.rows > p.cols;
+  const int small = (int)(turn ? p.cols : p.rows), large = (int)(turn ? p.rows : p.cols);
+  const int shares = shares_of(p.rows, p.cols);
+  MatList in = {}, out = {};
+  in.listed = out.listed = 1;
+  for (int i = 0; i < batch; ++i) {
+    in.at[i] = static_cast<char *>(const_cast<void *>(p.updates[first + i]));
+    out.at[i] = static_cast<char *>(p.outs[first + i]);
+  }
+  const int64_t rs = turn ? p.update_cs : p.update_rs, cs = turn ? p.update_rs : p.update_cs;
+  k_squares<<<dim3((unsigned)shares, (unsigned)batch), dim3(kSquareBlock), 0, s>>>(in, rs, cs, p.update_dtype, small, large,
+                                                                                 shares, r.squares);
+  ZEN_LAUNCH_CHECK("k_squares");
+  PackArgs pack = {};
+  pack.in = in;
+  pack.rs = rs;
+  pack.cs = cs;
+  pack.dtype = p.update_dtype;
+  pack.rows = small;
+  pack.cols = large;
+  pack.rows_all = (int)r.m;
+  pack.batch = batch;
+  pack.out = reinterpret_cast<uint16_t *>(r.x[0]);
+  pack.low = reinterpret_cast<uint16_t *>(r.x_low[0]);
+  pack.ld = r.n;
+  pack.out_batch = r.m * r.n;
+  pack.squares = r.squares;
+  pack.shares = shares;
+  pack.eps = p.eps;
+  pack.unit = kUnit;
+  if (const int rc = pack_matrices(pack, s)) return rc;
+
+  const int parts = p.precise ? 3 : 1;
+  const int m = (int)r.m, n = (int)r.n;
+  const int64_t mm = r.m * r.m, mn = r.m * r.n;
+  const MatSize gram = {m, m, n, 0, 0, batch, parts}, square = {m, m, m, 0, 0, batch, parts}, apply = {m, n, m, 0, 0, batch, parts};
+  for (int step = 0; step < p.steps; ++step) {
+    const int at = step & 1;
+    const bool near = step >= p.steps - 2;
+    const MatOperand x = operand(r.x[at], p.precise ? r.x_low[at] : nullptr, r.n, mn);
+    const MatOperand a = operand(r.a, r.a_low, r.m, mm), b = operand(r.b, r.b_low, r.m, mm);
+    KeepEpilogue e = {};
+    e.alpha = 1.f / kUnit;
+    e.d = r.a;
+    e.d_low = r.a_low;
+    e.d_ld = r.m;
+    e.d_batch = mm;
+    if (const int rc = launch_tiles<Tile, true, true, false, true>(gram, x, x, e, s)) return rc;
+    e.alpha = p.c / kUnit;
+    e.beta = p.b;
+    e.diag = near ? (p.a - 1.f) * kUnit : 0.f;
+    e.diag_n = small;
+    e.c = r.a;
+    e.c_low = r.a_low;
+    e.c_ld = r.m;
+    e.c_batch = mm;
+    e.d = r.b;
+    e.d_low = r.b_low;
+    if (const int rc = launch_tiles<Tile, true, true, false, true>(square, a, a, e, s)) return rc;
+    if (step + 1 < p.steps) {
+      e.alpha = 1.f / kUnit;
+      e.beta = near ? 1.f : p.a;
+      e.diag = 0.f;
+      e.c = r.x[at];
+      e.c_low = r.x_low[at];
+      e.d = r.x[at ^ 1];
+      e.d_low = r.x_low[at ^ 1];
+      e.c_ld = e.d_ld = r.n;
+      e.c_batch = e.d_batch = mn;
+      if (const int rc = launch_tiles<Tile, true, false, false, false>(apply, b, x, e, s)) return rc;
+      continue;
+    }
+    OutEpilogue o = {};
+    o.alpha = 1.f / (kUnit * kUnit);
+    o.beta = (near ? 1.f : p.a) / kUnit;
+    o.gain = p.weights ? -p.gain : 1.f;
+    o.keep = p.keep;
+    o.x = r.x[at];
+    o.x_low = r.x_low[at];
+    o.x_ld = r.n;
+    o.x_batch = mn;
+    o.rows = small;
+    o.cols = large;
+    o.out = out;
+    o.out_rs = turn ? p.out_cs : p.out_rs;
+    o.out_cs = turn ? p.out_rs : p.out_cs;
+    o.out_type = p.out_dtype;
+    o.res.listed = -1;
+    if (p.weights) {
+      o.res = o.out;
+      o.res_rs = o.out_rs;
+      o.res_cs = o.out_cs;
+      o.res_type = o.out_type;
+    }
+    if (const int rc = launch_tiles<Tile, true, false, false, false>(apply, b, x, o, s)) return rc;
+  }
+  return ZEN_OK;
+}
+
+constexpr int64_t kMostSide = kMostLd - 256;  // in whole tiles a row still has at most kMostLd elements
+
+}  // namespace
+}  // namespace zen
+
+extern "C" {
+
+size_t zen_orthogonal_workspace(int64_t rows, int64_t cols, int64_t count, int precise) {
+  using namespace zen;
+  if (rows <= 0 || cols <= 0 || count <= 0 || rows > kMostSide || cols > kMostSide) return 0;
+  return room_for(rows, cols, count, precise != 0, nullptr).bytes;
+}
+
+int zen_orthogonal(const zen_orthogonal_args *p) {
+  using namespace zen;
+  if (!p) return fail(ZEN_EINVAL, "zen_orthogonal: null pointer");
+  const auto known = [](int t) { return t == ZEN_F32 || t == ZEN_BF16 || t == ZEN_F16; };
+  if (!known(p->update_dtype) || !known(p->out_dtype)) return fail(ZEN_EINVAL, "zen_orthogonal: types are fp32, bf16 or fp16");
+  if (p->rows < 0 || p->cols < 0 || p->count < 0 || p->rows > kMostSide || p->cols > kMostSide)
+    return fail(ZEN_EINVAL, "zen_orthogonal: a size is out of range");
+  if (p->steps < 1) return fail(ZEN_EINVAL, "zen_orthogonal: at least one step");
+  if (!(p->eps >= 0)) return fail(ZEN_EINVAL, "zen_orthogonal: eps is not negative");
+  if (p->update_rs < 0 || p->update_cs < 0 || p->out_rs < 0 || p->out_cs < 0) return fail(ZEN_EINVAL, "zen_orthogonal: negative stride");
+  if (p->rows == 0 || p->cols == 0 || p->count == 0) return ZEN_OK;
+  if (!p->updates || !p->outs || !p->workspace) return fail(ZEN_EINVAL, "zen_orthogonal: null pointer");
+  for (int64_t i = 0; i < p->count; ++i)
+    if (!p->updates[i] || !p->outs[i]) return fail(ZEN_EINVAL, "zen_orthogonal: null pointer");
+  const Room r = room_for(p->rows, p->cols, p->count, p->precise != 0, p->workspace);
+  if (p->workspace_bytes < r.bytes) return fail(ZEN_EWORKSPACE, "zen_orthogonal: workspace too small");
+  for (int64_t first = 0; first < p->count; first += r.batch) {
+    const int64_t rest = p->count - first;
+    if (const int rc = chunk(*p, r, first, (int)(rest < r.batch ? rest : r.batch), static_cast<hipStream_t>(p->stream))) return rc;
+  }
+  return ZEN_OK;
+}
+
+}  // extern "C"
