@@ -328,6 +328,30 @@ def test_product(m, n, k, dtype, a_turned, b_turned):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [
+    (4200, 4100, 328), (2100, 4200, 72), (2000, 1500, 136), (1900, 1930, 2056),   # large tiles to small ones, one to some rounds
+    (512, 520, 4104), (70, 60, 8200), (1024, 300, 2056), (129, 129, 1000)])       # the steps of few tiles are shared
+@pytest.mark.parametrize("a_turned,b_turned", [(False, True), (False, False), (True, False)])
+def test_product_of_every_tile(m, n, k, a_turned, b_turned):
+    a = normal((k, m), 53, BF16).t() if a_turned else normal((m, k), 53, BF16)
+    b = normal((n, k), 54, BF16).t() if b_turned else normal((k, n), 54, BF16)
+    c = normal((m, n), 55, F16)
+    product_check(zen.product(a, b, residual=c, alpha=0.5, beta=3.0), a, b, c, 0.5, 3.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k", [(4100, 200), (3000, 136), (1000, 4104), (260, 2056)])
+def test_product_symmetric_of_every_tile(m, k):
+    a = normal((m, k), 56, F16)
+    out = zen.product(a, a.t(), symmetric=True, dtype=F32)
+    product_check(out, a, a.t(), None, 1.0, 0.0)
+    assert torch.equal(out, out.t())
+    out = zen.product(a, a.t(), symmetric=True)
+    assert out.dtype == F16 and torch.equal(out, out.t())
+    product_check(out, a, a.t(), None, 1.0, 0.0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("out", [BF16, F16, F32])
 @pytest.mark.parametrize("res", [BF16, F16, F32])
 def test_product_strides_types_and_the_residual_in_place(out, res):
@@ -478,7 +502,7 @@ def room_of(u, dtype, **more):
     return exact, U[dtype] + 2 * off(newton_schulz(u, half=True, **more), exact)
 
 
-SHAPES = [(1, 1), (1, 40), (3, 2), (64, 64), (65, 63), (128, 128), (48, 500), (500, 48), (200, 333), (300, 257), (130, 1030)]
+SHAPES = [(1, 1), (1, 40), (1100, 1030), (700, 2100), (3, 2), (64, 64), (65, 63), (128, 128), (48, 500), (500, 48), (200, 333), (300, 257), (130, 1030)]
 
 
 @pytest.mark.gpu

@@ -39,29 +39,32 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs p) {
     s_tile[i][j] = v;
   }
   __syncthreads();
-  uint16_t *out = p.out + (int64_t)z * p.out_batch;
-  uint16_t *low = p.low ? p.low + (int64_t)z * p.out_batch : nullptr;
+  const int64_t from = (int64_t)z * p.out_batch;
+  const auto write = [&](uint16_t *out, uint16_t *low, int64_t ld, int row0, int rows, int col0, bool turned) {
 #pragma unroll
-  for (int q = 0; q < kSide * kSide / 512; ++q) {  // two columns a lane
-    const int at = q * 256 + tid, j = (at & 31) * 2, i = at >> 5;
-    if (i0 + i >= p.rows_all || j0 + j >= p.ld) continue;
-    uint32_t word = 0, rest = 0;
+    for (int q = 0; q < kSide * kSide / 512; ++q) {  // two columns a lane
+      const int at = q * 256 + tid, j = (at & 31) * 2, i = at >> 5;
+      if (row0 + i >= rows || col0 + j >= ld) continue;
+      uint32_t word = 0, rest = 0;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const uint32_t raw = s_tile[i][j + e];
-      if (!p.squares) {
-        word |= raw << (16 * e);
-        continue;
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t raw = turned ? s_tile[j + e][i] : s_tile[i][j + e];
+        if (!p.squares) {
+          word |= raw << (16 * e);
+          continue;
+        }
+        const float v = (float)((double)__uint_as_float(raw) * scale);  // in fp64: a tiny update's scale is beyond fp32
+        const _Float16 h = (_Float16)v, l = (_Float16)(v - (float)h);
+        word |= (uint32_t)__builtin_bit_cast(uint16_t, h) << (16 * e);
+        rest |= (uint32_t)__builtin_bit_cast(uint16_t, l) << (16 * e);
       }
-      const float v = (float)((double)__uint_as_float(raw) * scale);  // in fp64: a tiny update's scale is beyond fp32
-      const _Float16 h = (_Float16)v, l = (_Float16)(v - (float)h);
-      word |= (uint32_t)__builtin_bit_cast(uint16_t, h) << (16 * e);
-      rest |= (uint32_t)__builtin_bit_cast(uint16_t, l) << (16 * e);
+      const int64_t to = from + (int64_t)(row0 + i) * ld + col0 + j;  // ld is even
+      *reinterpret_cast<uint32_t *>(out + to) = word;
+      if (low) *reinterpret_cast<uint32_t *>(low + to) = rest;
     }
-    const int64_t to = (int64_t)(i0 + i) * p.ld + j0 + j;  // ld is even
-    *reinterpret_cast<uint32_t *>(out + to) = word;
-    if (low) *reinterpret_cast<uint32_t *>(low + to) = rest;
-  }
+  };
+  write(p.out, p.low, p.ld, i0, p.rows_all, j0, false);
+  if (p.turned) write(p.turned, p.turned_low, p.rows_all, j0, (int)p.ld, i0, true);
 }
 
 }  // namespace

@@ -4,8 +4,6 @@
 namespace zen {
 namespace {
 
-using Tile = TileShape<128, 128, 2, 2>;
-
 // How an operand is read: its `rows` (of a, or columns of b) and k.
 struct Side {
   const void *p;
@@ -60,15 +58,17 @@ int lay_out(Side &s, int dtype, int64_t batches, Carver &cv, hipStream_t stream)
 bool known(int type) { return type == ZEN_F32 || type == ZEN_BF16 || type == ZEN_F16; }
 int64_t size_of(int type) { return type == ZEN_F32 ? 4 : 2; }
 
-template <bool AK, bool BK, bool BF, bool SYM>
-int go(const MatSize &size, const MatOperand &a, const MatOperand &b, const OutEpilogue &e, hipStream_t s) {
-  return launch_tiles<Tile, AK, BK, BF, SYM>(size, a, b, e, s);
+template <bool AK, bool BK>
+int go(const TilePlan &plan, float *partial, const MatSize &size, const MatOperand &a, const MatOperand &b, const OutEpilogue &e, bool bf,
+       bool sym, hipStream_t s) {
+  if (bf)
+    return sym ? run_tiles<AK, BK, true, true>(plan, partial, size, a, b, e, s) : run_tiles<AK, BK, true, false>(plan, partial, size, a, b, e, s);
+  return sym ? run_tiles<AK, BK, false, true>(plan, partial, size, a, b, e, s) : run_tiles<AK, BK, false, false>(plan, partial, size, a, b, e, s);
 }
 
-template <bool AK, bool BK>
-int go(const MatSize &size, const MatOperand &a, const MatOperand &b, const OutEpilogue &e, bool bf, bool sym, hipStream_t s) {
-  if (bf) return sym ? go<AK, BK, true, true>(size, a, b, e, s) : go<AK, BK, true, false>(size, a, b, e, s);
-  return sym ? go<AK, BK, false, true>(size, a, b, e, s) : go<AK, BK, false, false>(size, a, b, e, s);
+int lines(const void *p, int64_t rs, int64_t cs, int64_t batch, int type, int64_t batches) {
+  const int64_t size = size_of(type);
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && cs == 1 && rs * size % 16 == 0 && (batches <= 1 || batch * size % 16 == 0);
 }
 
 int check(const zen_product_args *p) {
@@ -84,6 +84,12 @@ int check(const zen_product_args *p) {
   return ZEN_OK;
 }
 
+Side side_a(const zen_product_args &p) { return side(p.a, p.a_rs, p.a_cs, p.a_batch, p.m, p.k, p.batch); }
+Side side_b(const zen_product_args &p) { return side(p.b, p.b_cs, p.b_rs, p.b_batch, p.n, p.k, p.batch); }
+TilePlan plan(const zen_product_args &p, const Side &a, const Side &b) {
+  return plan_tiles(p.m, p.n, p.k, 1, p.batch, p.symmetric != 0, a.contiguous && b.contiguous);
+}
+
 }  // namespace
 }  // namespace zen
 
@@ -92,8 +98,8 @@ extern "C" {
 size_t zen_product_workspace(const zen_product_args *p) {
   using namespace zen;
   if (check(p) != ZEN_OK || p->m == 0 || p->n == 0 || p->batch == 0 || p->k == 0) return 0;
-  return room(side(p->a, p->a_rs, p->a_cs, p->a_batch, p->m, p->k, p->batch), p->batch) +
-         room(side(p->b, p->b_cs, p->b_rs, p->b_batch, p->n, p->k, p->batch), p->batch);
+  const Side a = side_a(*p), b = side_b(*p);
+  return room(a, p->batch) + room(b, p->batch) + plan(*p, a, b).partial_bytes;
 }
 
 int zen_product(const zen_product_args *p) {
@@ -105,16 +111,17 @@ int zen_product(const zen_product_args *p) {
   if (need && !p->workspace) return fail(ZEN_EINVAL, "zen_product: null pointer");
   if (p->workspace_bytes < need) return fail(ZEN_EWORKSPACE, "zen_product: workspace too small");
   hipStream_t s = static_cast<hipStream_t>(p->stream);
-  Side sa = side(p->a, p->a_rs, p->a_cs, p->a_batch, p->m, p->k, p->batch);
-  Side sb = side(p->b, p->b_cs, p->b_rs, p->b_batch, p->n, p->k, p->batch);
+  Side sa = side_a(*p), sb = side_b(*p);
+  const TilePlan how = plan(*p, sa, sb);
+  Carver cv(p->workspace);
   if (p->k > 0) {
-    Carver cv(p->workspace);
     if (const int rc = lay_out(sa, p->dtype, p->batch, cv, s)) return rc;
     if (const int rc = lay_out(sb, p->dtype, p->batch, cv, s)) return rc;
   }
-  const MatSize size = {(int)p->m, (int)p->n, (int)p->k, 0, 0, (int)p->batch, 1};
-  MatOperand a = {{static_cast<const uint16_t *>(sa.p), nullptr}, sa.ld, sa.batch};
-  MatOperand b = {{static_cast<const uint16_t *>(sb.p), nullptr}, sb.ld, sb.batch};
+  const MatSize size = {(int)p->m, (int)p->n, (int)p->k, 0, 0, (int)p->batch, 1, 1, nullptr};
+  float *partial = reinterpret_cast<float *>(cv.base + cv.used);
+  const uint16_t *pa = static_cast<const uint16_t *>(sa.p), *pb = static_cast<const uint16_t *>(sb.p);
+  const MatOperand a = {{pa, pa}, sa.ld, sa.batch}, b = {{pb, pb}, sb.ld, sb.batch};
   OutEpilogue e = {};
   e.alpha = p->alpha;
   e.gain = 1.f;
@@ -126,8 +133,10 @@ int zen_product(const zen_product_args *p) {
   e.out_rs = p->out_rs;
   e.out_cs = p->out_cs;
   e.out_type = p->out_dtype;
+  e.lines = lines(p->out, p->out_rs, p->out_cs, p->out_batch, p->out_dtype, p->batch);
   e.res.listed = -1;
   if (p->c) {
+    e.lines &= lines(p->c, p->c_rs, p->c_cs, p->c_batch, p->c_dtype, p->batch);
     e.res.listed = 0;
     e.res.base = static_cast<char *>(const_cast<void *>(p->c));
     e.res.stride = p->c_batch * size_of(p->c_dtype);
@@ -137,8 +146,8 @@ int zen_product(const zen_product_args *p) {
   }
   const bool bf = p->dtype == ZEN_BF16, sym = p->symmetric != 0;
   if (sa.contiguous)
-    return sb.contiguous ? go<true, true>(size, a, b, e, bf, sym, s) : go<true, false>(size, a, b, e, bf, sym, s);
-  return sb.contiguous ? go<false, true>(size, a, b, e, bf, sym, s) : go<false, false>(size, a, b, e, bf, sym, s);
+    return sb.contiguous ? go<true, true>(how, partial, size, a, b, e, bf, sym, s) : go<true, false>(how, partial, size, a, b, e, bf, sym, s);
+  return sb.contiguous ? go<false, true>(how, partial, size, a, b, e, bf, sym, s) : go<false, false>(how, partial, size, a, b, e, bf, sym, s);
 }
 
 }  // extern "C"

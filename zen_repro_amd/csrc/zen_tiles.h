@@ -1,17 +1,22 @@
 // Matrix products in tiles, for zen_product.hip and zen_orthogonal.hip.
 //
-//   D[i, j] = sum over k of A[i, k] B[k, j],   A and B in 16 bits, sums in fp32 (MFMA 16x16x32)
+//   D[i, j] = sum over k of A[i, k] B[k, j],   A and B in 16 bits, sums in fp32 (MFMA 32x32x16)
 //
 // A workgroup owns a tile of D and walks k in steps of 64.  A step's pieces of A and B come straight into LDS (buffer
-// loads with an LDS destination, 16 bytes a lane); two buffers take turns, so a step's loads are in flight while the step before
-// it is multiplied.  Each operand may be stored with k contiguous (rows of k) or with k as the stride (rows of i or j):
+// loads with an LDS destination, 16 bytes a lane) into buffers that go round, so the loads of the steps ahead are in flight while
+// one is multiplied.  Each operand may be stored with k contiguous (rows of k) or with k as the stride (rows of i or j):
 // the first is read from LDS 16 bytes a lane, the second by transposing reads (ds_read_b64_tr_b16), so no operand is ever
 // transposed in memory.  The range check of the buffer loads puts zeros where the tile hangs over the operand's end.
 //
-// LDS layout: a row of 64 k is eight 16-byte pieces; the piece k / 8 of row r lies in place (k / 8) ^ (r & 7), which
-// spreads the eight rows that eight lanes read at once over all banks.  With k as the stride a row holds the tile's i or j,
-// and piece c of row k lies in place c ^ ((k & 3) << 1): the four rows that sixteen lanes of a transposing read take lie
-// in different banks.  The loads' LDS destination is one run of lanes, so the swizzle is in the addresses they read from.
+// What bounds it: with 256 x 256 tiles a step's products take a compute unit 2048 cycles, of some 2900 (8192^3, k contiguous:
+// matrix cores busy 71 % of the cycles, LDS 20 %, and a clock that the power limit holds at 1.5 to 1.9 GHz: 1110 to 1260
+// TFLOP/s; without the loads, 1550).  What mattered most: reads, loads and products in an order of our own, one by one (the
+// compiler's: 1.83 against 1.50 million cycles at that size), and reads of LDS without bank conflicts.
+//
+// LDS layout: a row of 64 k is eight 16-byte pieces; piece c of row r lies in place c ^ key(r).  With k as the stride a row
+// holds the tile's i or j, and piece c of row k lies in place(k, c).  Both spread what lanes read at the same time (32 rows at one c;
+// four rows of k at two or four neighbouring pieces) over all banks: no conflicts were counted.  The loads' LDS destination is one run
+// of lanes, so the order is in the addresses they read from.
 #pragma once
 
 #include "zen_common.h"
@@ -23,13 +28,14 @@ typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef short short8v __attribute__((ext_vector_type(8)));
 typedef float float4v __attribute__((ext_vector_type(4)));
+typedef float float16v __attribute__((ext_vector_type(16)));
 
 constexpr int kTileK = 64;
 constexpr int64_t kMostLd = 1 << 21;  // a step's addresses, 256 rows at most, stay below 2^30
 constexpr int kMostList = 32;  // matrices of separate addresses to a launch
 
 struct MatOperand {
-  const uint16_t *p[2];  // the matrix, and (split products) what its rounding to 16 bits left over
+  const uint16_t *p[2];  // the matrix, and what its rounding to 16 bits left over (itself where there is nothing: never null)
   int64_t ld;            // elements from row to row
   int64_t batch;         // elements from matrix to matrix
 };
@@ -38,7 +44,9 @@ struct MatSize {
   int m, n, k;
   int tiles_m, tiles_n;
   int batch;
-  int parts;  // 1: A B; 3: A B + A B' + A' B with the left-overs A', B'
+  int parts;       // 1: A B; 3: A B + A B' + A' B with the left-overs A', B'
+  int splits;      // > 1: the steps of a tile are shared among so many workgroups, whose sums go to `partial`
+  float *partial;  // and are joined by a launch of their own
 };
 
 // Addresses of a stack's matrices: base + b * stride, or a list.
@@ -50,13 +58,15 @@ struct MatList {
   __device__ __forceinline__ char *of(int b) const { return listed ? at[b] : base + (int64_t)b * stride; }
 };
 
-template <int BM_, int BN_, int WM_, int WN_>
+template <int BM_, int BN_, int WM_, int WN_, int STAGES>
 struct TileShape {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;       // tile, waves down and across
   static constexpr int W = WM * WN, threads = W * 64;
   static constexpr int TM = BM / WM, TN = BN / WN;                   // a wave's part
-  static constexpr int FM = TM / 16, FN = TN / 16;                   // its MFMA blocks
-  static constexpr int stage_bytes = (BM + BN) * kTileK * 2;
+  static constexpr int FM = TM / 32, FN = TN / 32;                   // its MFMA blocks
+  static constexpr int stages = STAGES;                              // buffers that go round
+  static constexpr int stage_halves = (BM + BN) * kTileK;
+  static constexpr int wave_sums = TM * TN;
 };
 
 #define ZEN_LDS __attribute__((address_space(3)))
@@ -69,58 +79,61 @@ struct TileOperand {
   static constexpr int row_lanes = KC ? 8 : R / 8;    // lanes to a row of the piece
   static constexpr int rows = 64 / row_lanes;         // rows to a load
   static_assert(KC || (W * rows) % 4 == 0, "the swizzle is the same in every load of a wave");
-  const char *base;      // of the next step
-  int64_t left;          // bytes of the operand from there on
-  int64_t step;          // bytes to the next step
-  uint32_t voffset, soffset;
+  const char *first[2];  // of the tile in the matrix, and in what its rounding left over
+  int64_t all;           // bytes of the operand from there on
+  int64_t step;          // bytes from step to step
+  uint32_t voffset, soffset, vnow;
+  __amdgpu_buffer_rsrc_t source;
   int tail_chunk;        // KC: this lane's first k within the step
 
+  // k contiguous: piece c of row r lies in place c ^ key(r)
+  static __device__ __forceinline__ int key(int r) { return ((r >> 1) & 3) | ((r >> 2) & 4); }
+
+  // k as the stride: where piece `chunk` of row k of the step lies
+  static __device__ __forceinline__ int place(int k, int chunk) { return chunk ^ (R >= 128 ? (k & 3) << 2 : (k & 2) << 1); }
+
   // r0: first row (i or j) of the tile; rows_all: rows there are; k: the operand's k
-  __device__ __forceinline__ void start(const uint16_t *p, int64_t ld, int64_t r0, int64_t rows_all, int k, int wave, int lane) {
+  __device__ __forceinline__ void start(const MatOperand &o, int z, int64_t r0, int64_t rows_all, int k, int wave, int lane) {
     const int row = wave * rows + lane / row_lanes;
     const int slot = lane % row_lanes;
-    if (KC) {
-      const int chunk = slot ^ (row & 7);
-      tail_chunk = chunk * 8;
-      base = reinterpret_cast<const char *>(p + r0 * ld);
-      left = ((rows_all - r0 - 1) * ld + ((k + 7) & ~7)) * 2;  // whole pieces: k is a multiple of 8, or ld has room
-      voffset = (uint32_t)((row * ld + chunk * 8) * 2);
-      step = kTileK * 2;
-    } else {
-      const int chunk = slot ^ ((row & 3) << 1);
-      tail_chunk = 0;
-      base = reinterpret_cast<const char *>(p + r0);
-      left = (((int64_t)k - 1) * ld + ((rows_all - r0 + 1) & ~1ll)) * 2;  // whole words: the address is a multiple of 16
-      voffset = (uint32_t)((row * ld + chunk * 8) * 2);
-      step = kTileK * ld * 2;
-    }
+    const int chunk = KC ? slot ^ key(row) : place(row, slot);
+    const int64_t ld = o.ld, from = z * o.batch + (KC ? r0 * ld : r0);
+    first[0] = reinterpret_cast<const char *>(o.p[0] + from);
+    first[1] = reinterpret_cast<const char *>(o.p[1] + from);
+    tail_chunk = chunk * 8;
+    voffset = (uint32_t)((row * ld + chunk * 8) * 2);
+    // whole pieces: k is a multiple of 8, or ld has room; whole words: the address is a multiple of 16
+    all = KC ? ((rows_all - r0 - 1) * ld + ((k + 7) & ~7)) * 2 : (((int64_t)k - 1) * ld + ((rows_all - r0 + 1) & ~1ll)) * 2;
+    step = KC ? kTileK * 2 : kTileK * ld * 2;
     soffset = (uint32_t)(W * rows * ld * 2);
   }
 
-  // The loads of the step at `base`, whose first k is k0 of k, into `lds` (this operand's part of a buffer).
-  __device__ __forceinline__ void load(uint16_t *lds, int k0, int k, int wave) {
+  // What the loads of step `at` (of `low`'s matrix) read: nothing where `there` is false (zeros arrive).
+  __device__ __forceinline__ void aim(int at, bool low, bool there, int k) {
     const int64_t most = 0x7fff0000ll;  // the addresses of a tile end below (kMostLd)
+    const int64_t left = there ? all - at * step : 0;
     const uint32_t records = left <= 0 ? 0u : (uint32_t)(left < most ? left : most);
-    auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, (int)records, 0x00027000);
-    const uint32_t vo = KC && k0 + kTileK > k && k0 + tail_chunk >= k ? 0x80000000u : voffset;
-#pragma unroll
-    for (int q = 0; q < loads; ++q)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (ZEN_LDS void *)(lds + (q * W + wave) * 512), 16, (int)vo,
-                                               (int)(q * soffset), 0, 0);
-    base += step;
-    left -= step;
+    source = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(first[low] + at * step), 0, (int)records, 0x00027000);
+    vnow = KC && at * kTileK + tail_chunk >= k ? 0x80000000u : voffset;
   }
 
-  // The block of sixteen rows from row r0 of the tile (a multiple of 16) and k from kk * 32, as an MFMA operand.
+  // Load q of them into `lds` (this operand's part of a buffer).
+  __device__ __forceinline__ void load(uint16_t *lds, int q, int wave) const {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(source, (ZEN_LDS void *)(lds + (q * W + wave) * 512), 16, (int)vnow,
+                                             (int)(q * soffset), 0, 0);
+  }
+
+  // The block of 32 rows from row r0 of the tile (a multiple of 32) and k from kk * 16, as an MFMA operand.
   static __device__ __forceinline__ short8v read(const uint16_t *lds, int r0, int kk, int lane) {
     if (KC) {
-      const int r = r0 + (lane & 15);
-      const int chunk = (kk * 4 + (lane >> 4)) ^ (lane & 7);
+      const int r = r0 + (lane & 31);
+      const int chunk = (kk * 2 + (lane >> 5)) ^ key(lane);  // r0 is a multiple of 32
       return *reinterpret_cast<const short8v *>(lds + r * kTileK + chunk * 8);
     }
+    // sixteen lanes turn four rows of sixteen: lane j gives the address of four elements of row j / 4
     const int j = lane & 15;
-    const int krow = kk * 32 + (lane >> 4) * 8 + (j >> 2);
-    const int slot = ((r0 >> 3) ^ ((j >> 2) << 1)) + ((j & 3) >> 1);
+    const int krow = kk * 16 + (lane >> 5) * 8 + (j >> 2);
+    const int slot = place(krow, (r0 >> 3) + ((lane >> 4) & 1) * 2 + ((j & 3) >> 1));  // the same four rows on
     const uint16_t *at = lds + krow * R + slot * 8 + (j & 1) * 4;
     const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ZEN_LDS short4v *)(at));
     const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ZEN_LDS short4v *)(at + 4 * R));
@@ -128,11 +141,23 @@ struct TileOperand {
   }
 };
 
+// All but the newest LOADS of the wave's loads into LDS have arrived, it has got what it read from there, and so have all waves of
+// the workgroup.  (A fence would wait for all loads.)
+template <int LOADS>
+__device__ __forceinline__ void arrived() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x70 | (LOADS & 15) | (LOADS >> 4) << 14);  // vmcnt(LOADS) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 template <bool BF>
-__device__ __forceinline__ float4v mfma(short8v a, short8v b, float4v c) {
+__device__ __forceinline__ float16v mfma(short8v a, short8v b, float16v c) {
   if (BF)
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
 }
 
 // Row and column of tile t of the lower triangle, counted row by row.
@@ -143,15 +168,23 @@ __device__ __forceinline__ void triangle(int t, int &i, int &j) {
   j = t - (int)((int64_t)i * (i + 1) / 2);
 }
 
-// The launch's tiles: of the whole matrix, or of its lower triangle (SYM).  Workgroups go round the eight dies, whose
+// Number of a tile among the launch's, for what is kept by tiles.
+template <bool SYM>
+__device__ __forceinline__ int tile_number(const MatSize &s, int b, int ti, int tj) {
+  return SYM ? b * (s.tiles_m * (s.tiles_m + 1) / 2) + ti * (ti + 1) / 2 + tj : (b * s.tiles_m + ti) * s.tiles_n + tj;
+}
+
+// The launch's tiles: of the whole matrix, or of its lower triangle (SYM), each in so many shares.  Workgroups go round the eight dies, whose
 // L2s are apart: the tiles are dealt so that a die's are neighbours, four tile rows by all columns at a time.
 template <bool SYM>
-__device__ __forceinline__ void tile_of(const MatSize &s, int &b, int &ti, int &tj) {
+__device__ __forceinline__ void tile_of(const MatSize &s, int shares, int &share, int &b, int &ti, int &tj) {
   const int per = SYM ? s.tiles_m * (s.tiles_m + 1) / 2 : s.tiles_m * s.tiles_n;
-  const int all = per * s.batch;
+  const int all = per * s.batch * shares;
   int t = (int)blockIdx.x;
   const int die = t & 7, most = all >> 3, rest = all & 7;
   t = die * most + (die < rest ? die : rest) + (t >> 3);
+  share = t % shares;
+  t /= shares;
   b = t / per;
   t -= b * per;
   if (SYM) {
@@ -166,87 +199,7 @@ __device__ __forceinline__ void tile_of(const MatSize &s, int &b, int &ti, int &
   tj = t / rows;
 }
 
-template <class S, bool AK, bool BK, bool BF, bool SYM, class Epilogue>
-__global__ __launch_bounds__(S::threads, 2) void k_tiles(MatSize size, MatOperand a, MatOperand b, Epilogue epilogue) {
-  __shared__ __attribute__((aligned(1024))) uint16_t s_buf[S::stage_bytes];
-  int z, ti, tj;
-  tile_of<SYM>(size, z, ti, tj);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / S::WN, wn = wave % S::WN;
-  using OpA = TileOperand<S::BM, AK, S::W>;
-  using OpB = TileOperand<S::BN, BK, S::W>;
-  OpA la;
-  OpB lb;
-  const int steps = (size.k + kTileK - 1) / kTileK, all = steps * size.parts;
-  int at = 0, part = 0;  // what is loaded next: step of a part
-
-  auto next = [&](uint16_t *buf) {
-    if (at == 0) {
-      la.start(a.p[part == 2] + z * a.batch, a.ld, (int64_t)ti * S::BM, size.m, size.k, wave, lane);
-      lb.start(b.p[part == 1] + z * b.batch, b.ld, (int64_t)tj * S::BN, size.n, size.k, wave, lane);
-    }
-    la.load(buf, at * kTileK, size.k, wave);
-    lb.load(buf + S::BM * kTileK, at * kTileK, size.k, wave);
-    if (++at == steps) {
-      at = 0;
-      ++part;
-    }
-  };
-
-  float4v acc[S::FM][S::FN];
-#pragma unroll
-  for (int i = 0; i < S::FM; ++i)
-#pragma unroll
-    for (int j = 0; j < S::FN; ++j) acc[i][j] = float4v{0.f, 0.f, 0.f, 0.f};
-
-  auto multiply = [&](const uint16_t *buf) {
-#pragma unroll
-    for (int kk = 0; kk < kTileK / 32; ++kk) {
-      __builtin_amdgcn_sched_barrier(0);
-      short8v fa[S::FM], fb[S::FN];
-#pragma unroll
-      for (int i = 0; i < S::FM; ++i) fa[i] = OpA::read(buf, wm * S::TM + i * 16, kk, lane);
-#pragma unroll
-      for (int j = 0; j < S::FN; ++j) fb[j] = OpB::read(buf + S::BM * kTileK, wn * S::TN + j * 16, kk, lane);
-#pragma unroll
-      for (int i = 0; i < S::FM; ++i)
-#pragma unroll
-        for (int j = 0; j < S::FN; ++j) acc[i][j] = mfma<BF>(fb[j], fa[i], acc[i][j]);
-    }
-  };
-
-  // A buffer is loaded again only behind the barrier that every wave reaches after its reads of it.
-  if (all > 0) next(s_buf);
-  int turn = 0;
-  for (int t = 0; t < all; ++t) {
-    __builtin_amdgcn_s_waitcnt(0xf70);  // vmcnt(0): this wave's loads are in LDS
-    __syncthreads();
-    if (t + 1 < all) next(s_buf + (turn ^ (S::stage_bytes / 2)));
-    multiply(s_buf + turn);
-    turn ^= S::stage_bytes / 2;
-  }
-
-  // A lane holds four neighbours of a row: row lane & 15 of a block, columns (lane >> 4) * 4 and on.
-  const int row0 = ti * S::BM + wm * S::TM + (lane & 15), col0 = tj * S::BN + wn * S::TN + (lane >> 4) * 4;
-#pragma unroll
-  for (int i = 0; i < S::FM; ++i)
-#pragma unroll
-    for (int j = 0; j < S::FN; ++j) epilogue.put(z, row0 + i * 16, col0 + j * 16, acc[i][j], SYM && ti != tj);
-}
-
-template <class S, bool AK, bool BK, bool BF, bool SYM, class Epilogue>
-inline int launch_tiles(MatSize size, const MatOperand &a, const MatOperand &b, const Epilogue &e, hipStream_t stream) {
-  size.tiles_m = (size.m + S::BM - 1) / S::BM;
-  size.tiles_n = (size.n + S::BN - 1) / S::BN;
-  const int64_t per = SYM ? (int64_t)size.tiles_m * (size.tiles_m + 1) / 2 : (int64_t)size.tiles_m * size.tiles_n;
-  const int64_t blocks = per * size.batch;
-  if (blocks > 0x7fffffffll) return fail(ZEN_EINVAL, "matrix product: too many tiles");
-  k_tiles<S, AK, BK, BF, SYM, Epilogue><<<dim3((unsigned)blocks), dim3(S::threads), 0, stream>>>(size, a, b, e);
-  ZEN_LAUNCH_CHECK("k_tiles");
-  return ZEN_OK;
-}
-
-// ---------------------------------------------------------------- values of three types
+// ---------------------------------------------------------------- what becomes of a tile
 
 __device__ __forceinline__ float load_value(const char *p, int64_t i, int dtype) {
   if (dtype == ZEN_F32) return reinterpret_cast<const float *>(p)[i];
@@ -260,79 +213,445 @@ __device__ __forceinline__ void store_value(char *p, int64_t i, int dtype, float
   else reinterpret_cast<_Float16 *>(p)[i] = (_Float16)v;
 }
 
+typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+typedef float float8v __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ float8v widen(half8v v) { return __builtin_convertvector(v, float8v); }
+
+__device__ __forceinline__ float8v load_eight(const char *p, int64_t i, int dtype) {
+  if (dtype == ZEN_F32) return *reinterpret_cast<const float8v *>(p + i * 4);
+  if (dtype == ZEN_BF16) return __builtin_convertvector(*reinterpret_cast<const bf8 *>(p + i * 2), float8v);
+  return widen(*reinterpret_cast<const half8v *>(p + i * 2));
+}
+
+__device__ __forceinline__ void store_eight(char *p, int64_t i, int dtype, float8v v) {
+  if (dtype == ZEN_F32) *reinterpret_cast<float8v *>(p + i * 4) = v;
+  else if (dtype == ZEN_BF16) *reinterpret_cast<bf8 *>(p + i * 2) = __builtin_convertvector(v, bf8);
+  else *reinterpret_cast<half8v *>(p + i * 2) = __builtin_convertvector(v, half8v);
+}
+
+// The wave's order of its own LDS operations is the program's; this holds the compiler to it.
+__device__ __forceinline__ void lds_in_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// 32 rows of a wave's sums on their way out, through LDS: written as the MFMA layout has them, read eight neighbours a lane,
+// of a row or (for a mirror image) of a column.  Rows of COLS + 4: neighbouring rows begin in different banks.
+template <int COLS>
+struct Stage {
+  static constexpr int row = COLS + 4;
+  static constexpr int floats = 32 * row;
+  static constexpr int turns = 32 * COLS / 512;  // eight a lane
+
+  static __device__ __forceinline__ void of_row(int turn, int lane, int &i, int &j) {
+    const int at = turn * 64 + lane;
+    i = at / (COLS / 8);
+    j = at % (COLS / 8) * 8;
+  }
+  static __device__ __forceinline__ float8v row_sums(const float *sums, int i, int j) {
+    const float4v a = *reinterpret_cast<const float4v *>(sums + i * row + j), b = *reinterpret_cast<const float4v *>(sums + i * row + j + 4);
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  static __device__ __forceinline__ void put_row(float *sums, int i, int j, float8v v) {
+    *reinterpret_cast<float4v *>(sums + i * row + j) = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+    *reinterpret_cast<float4v *>(sums + i * row + j + 4) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+  }
+  static __device__ __forceinline__ void of_column(int turn, int lane, int &i, int &j) {
+    const int at = turn * 64 + lane;
+    i = (at & 3) * 8;
+    j = at >> 2;
+  }
+  static __device__ __forceinline__ float8v column_sums(const float *sums, int i, int j) {
+    float8v v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = sums[(i + e) * row + j];
+    return v;
+  }
+};
+
 // What goes out to a caller's matrix: out = gain * (alpha * acc + beta * (X + X')) + keep * res.
 struct OutEpilogue {
   float alpha, beta, gain, keep;
-  const _Float16 *x, *x_low;  // null: none
+  const _Float16 *x, *x_low;  // null: none (and no mirror image where there is one)
   int64_t x_ld, x_batch;
   int rows, cols;
   MatList out, res;             // res: listed < 0 for none
   int64_t out_rs, out_cs, res_rs, res_cs;
   int out_type, res_type;
+  int lines;                    // rows of out and res are contiguous and begin at multiples of 16 bytes
 
-  __device__ __forceinline__ void one(char *o, const char *r, int i, int j, float v) const {
-    if (res.listed >= 0) v = gain * v + keep * load_value(r, i * res_rs + j * res_cs, res_type);
-    else v *= gain;
-    store_value(o, i * out_rs + j * out_cs, out_type, v);
-  }
-
-  __device__ __forceinline__ void put(int z, int i, int j, float4v acc, bool mirror) const {
-    if (i >= rows) return;
+  template <int COLS>
+  __device__ __forceinline__ void block(int z, int i0, int j0, float *sums, bool mirror, int lane) const {
+    using T = Stage<COLS>;
     char *o = out.of(z);
     const char *r = res.listed >= 0 ? res.of(z) : nullptr;
+    if (lines && i0 + 32 <= rows && j0 + COLS <= cols) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (j + e >= cols) break;
-      float v = alpha * acc[e];
-      if (x) {
-        const int64_t at = z * x_batch + (int64_t)i * x_ld + j + e;
-        v += beta * ((float)x[at] + (float)x_low[at]);
+      for (int turn = 0; turn < T::turns; ++turn) {
+        int i, j;
+        T::of_row(turn, lane, i, j);
+        float8v v = alpha * T::row_sums(sums, i, j);
+        i += i0;
+        j += j0;
+        if (x) {
+          const int64_t at = z * x_batch + (int64_t)i * x_ld + j;
+          v += beta * (widen(*reinterpret_cast<const half8v *>(x + at)) + widen(*reinterpret_cast<const half8v *>(x_low + at)));
+        }
+        v *= gain;
+        if (r) v += keep * load_eight(r, i * res_rs + j, res_type);
+        store_eight(o, i * out_rs + j, out_type, v);
       }
-      one(o, r, i, j + e, v);
-      if (mirror) one(o, r, j + e, i, v);
+      if (!mirror) return;
+#pragma unroll 1
+      for (int turn = 0; turn < T::turns; ++turn) {
+        int i, j;
+        T::of_column(turn, lane, i, j);
+        float8v v = gain * alpha * T::column_sums(sums, i, j);
+        i += i0;
+        j += j0;
+        if (r) v += keep * load_eight(r, j * res_rs + i, res_type);
+        store_eight(o, j * out_rs + i, out_type, v);
+      }
+      return;
+    }
+    // one by one: the tile hangs over the matrix, or its rows are not lines
+    const int turns = mirror ? 2 : 1;
+    for (int turn = 0; turn < turns; ++turn) {
+#pragma unroll 2
+      for (int at = lane; at < 32 * COLS; at += 64) {
+        const int di = turn ? at & 31 : at / COLS, dj = turn ? at >> 5 : at % COLS;
+        const int i = i0 + di, j = j0 + dj;
+        if (i >= rows || j >= cols) continue;
+        float v = alpha * sums[di * T::row + dj];
+        if (x) {
+          const int64_t from = z * x_batch + (int64_t)i * x_ld + j;
+          v += beta * ((float)x[from] + (float)x_low[from]);
+        }
+        v *= gain;
+        const int64_t to_i = turn ? j : i, to_j = turn ? i : j;
+        if (r) v += keep * load_value(r, to_i * res_rs + to_j * res_cs, res_type);
+        store_value(o, to_i * out_rs + to_j * out_cs, out_type, v);
+      }
     }
   }
 };
 
-// What goes back to a workspace: d = alpha * acc + beta * (c + c') + diag on the diagonal, in one or two times 16 bits.
+// What goes back to a workspace: d = alpha * acc + beta * (c + c') + diag on the diagonal, in one or two times 16 bits, and
+// (t not null) its transpose beside it.  Rows and columns are multiples of 64.
 struct KeepEpilogue {
   float alpha, beta, diag;
+  int rows, cols;
   int diag_n;  // the diagonal's length
   const _Float16 *c, *c_low;
-  _Float16 *d, *d_low;
-  int64_t c_ld, c_batch, d_ld, d_batch;
+  _Float16 *d, *d_low, *t, *t_low;
+  int64_t ld, batch, t_ld, t_batch;  // c lies as d does
 
-  __device__ __forceinline__ void put(int z, int i, int j, float4v acc, bool mirror) const {
+  static __device__ __forceinline__ void store(_Float16 *p, _Float16 *low, int64_t at, float8v v) {
+    const half8v h = __builtin_convertvector(v, half8v);
+    *reinterpret_cast<half8v *>(p + at) = h;
+    if (low) *reinterpret_cast<half8v *>(low + at) = __builtin_convertvector(v - widen(h), half8v);
+  }
+
+  template <int COLS>
+  __device__ __forceinline__ void block(int z, int i0, int j0, float *sums, bool mirror, int lane) const {
+    using T = Stage<COLS>;
+    if (i0 >= rows || j0 >= cols) return;
+    const bool turned = mirror || t;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float v = alpha * acc[e];
-      if (c) {
-        const int64_t at = z * c_batch + (int64_t)i * c_ld + j + e;
-        v += beta * ((float)c[at] + (c_low ? (float)c_low[at] : 0.f));
+    for (int turn = 0; turn < T::turns; ++turn) {
+      int di, dj;
+      T::of_row(turn, lane, di, dj);
+      const int i = i0 + di, j = j0 + dj;
+      const int64_t at = z * batch + (int64_t)i * ld + j;
+      float8v v = alpha * T::row_sums(sums, di, dj);
+      if (c) v += beta * widen(*reinterpret_cast<const half8v *>(c + at));
+      if (c_low) v += beta * widen(*reinterpret_cast<const half8v *>(c_low + at));
+      if (diag != 0.f && i >= j && i < j + 8 && i < diag_n) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += i == j + e ? diag : 0.f;
       }
-      if (i == j + e && i < diag_n) v += diag;
-      const _Float16 h = (_Float16)v, l = (_Float16)(v - (float)h);
-      const int64_t at = z * d_batch + (int64_t)i * d_ld + j + e, to = z * d_batch + (int64_t)(j + e) * d_ld + i;
-      d[at] = h;
-      if (d_low) d_low[at] = l;
-      if (mirror) {
-        d[to] = h;
-        if (d_low) d_low[to] = l;
-      }
+      store(d, d_low, at, v);
+      if (turned) T::put_row(sums, di, dj, v);
+    }
+    if (!turned) return;
+    lds_in_order();
+    _Float16 *to = mirror ? d : t, *to_low = mirror ? d_low : t_low;
+    const int64_t to_ld = mirror ? ld : t_ld, from = z * (mirror ? batch : t_batch);
+#pragma unroll
+    for (int turn = 0; turn < T::turns; ++turn) {
+      int di, dj;
+      T::of_column(turn, lane, di, dj);
+      store(to, to_low, from + (int64_t)(j0 + dj) * to_ld + i0 + di, T::column_sums(sums, di, dj));
     }
   }
 };
+
+// LDS of a wave's epilogue, in halves.
+template <class S>
+constexpr int epilogue_cols() { return S::TN % 64 ? 32 : 64; }
+template <class S>
+constexpr int epilogue_halves() { return 2 * Stage<epilogue_cols<S>()>::floats; }
+
+// A wave's part of the tile, from row i0 and column j0 on.
+template <class S, class Epilogue>
+__device__ __forceinline__ void finish(const Epilogue &e, int z, int i0, int j0, const float16v (&acc)[S::FM][S::FN], bool mirror,
+                                       uint16_t *lds, int lane) {
+  constexpr int kCols = epilogue_cols<S>();
+  float *sums = reinterpret_cast<float *>(lds);
+#pragma unroll
+  for (int a = 0; a < S::FM; ++a)
+#pragma unroll
+    for (int c = 0; c < S::TN; c += kCols) {
+      // of a 32 x 32 block a lane holds row lane & 31: four times four neighbours, eight columns apart
+#pragma unroll
+      for (int b = 0; b < kCols / 32; ++b)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float16v &f = acc[a][c / 32 + b];
+          *reinterpret_cast<float4v *>(sums + (lane & 31) * Stage<kCols>::row + b * 32 + q * 8 + (lane >> 5) * 4) =
+              float4v{f[q * 4], f[q * 4 + 1], f[q * 4 + 2], f[q * 4 + 3]};
+        }
+      lds_in_order();
+      e.template block<kCols>(z, i0 + a * 32, j0 + c, sums, mirror, lane);
+      lds_in_order();
+    }
+}
+
+template <class S, bool AK, bool BK, bool BF, bool SYM, class Epilogue>
+__global__ __launch_bounds__(S::threads, S::W > 4 || S::stages * S::stage_halves <= 40960 ? 2 : 1) void k_tiles(MatSize size, MatOperand a, MatOperand b, Epilogue epilogue) {
+  static_assert(S::W * epilogue_halves<S>() <= S::stages * S::stage_halves, "the epilogue fits the buffers");
+  __shared__ __attribute__((aligned(1024))) uint16_t s_buf[S::stages * S::stage_halves];
+  int z, ti, tj, share;
+  tile_of<SYM>(size, size.splits, share, z, ti, tj);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / S::WN, wn = wave % S::WN;
+  using OpA = TileOperand<S::BM, AK, S::W>;
+  using OpB = TileOperand<S::BN, BK, S::W>;
+  OpA la;
+  OpB lb;
+  const int steps = (size.k + kTileK - 1) / kTileK;
+  // this workgroup's steps of all parts
+  const int begin = (int)((int64_t)steps * size.parts * share / size.splits);
+  const int all = (int)((int64_t)steps * size.parts * (share + 1) / size.splits) - begin;
+  la.start(a, z, (int64_t)ti * S::BM, size.m, size.k, wave, lane);
+  lb.start(b, z, (int64_t)tj * S::BN, size.n, size.k, wave, lane);
+  int at = begin % (steps ? steps : 1), part = begin / (steps ? steps : 1);  // what is loaded next: step of a part
+  int left = all;
+
+  auto aim = [&]() {  // no branches: the loads are to lie between the products
+    const bool there = left-- > 0;
+    la.aim(at, there && part == 2, there, size.k);
+    lb.aim(at, there && part == 1, there, size.k);
+    const bool wrap = at + 1 == steps;
+    at = wrap ? 0 : at + 1;
+    part += wrap;
+  };
+  constexpr int kLoads = OpA::loads + OpB::loads;
+  auto load = [&](uint16_t *buf, int l) {
+    if (l < OpA::loads) la.load(buf, l, wave);
+    else lb.load(buf + S::BM * kTileK, l - OpA::loads, wave);
+  };
+
+  float16v acc[S::FM][S::FN];
+#pragma unroll
+  for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) acc[i][j] = float16v{};
+
+  // Fragments of 16 k are read while those before them are multiplied, also across the steps: a step's last quarter is
+  // multiplied while the first of the next one is read.  In front of that lies the step's one barrier: every wave has
+  // read all of the step's buffer and its own loads of the next one have arrived; behind it the buffer is loaded again, in
+  // this quarter and the next.  Reads and loads lie one by one between the products (a row of loads would hold the wave up for
+  // as long as the address unit takes over them), in the order written here.
+  short8v fa[2][S::FM], fb[2][S::FN];
+  constexpr int kProducts = S::FM * S::FN, kReads = S::FM + S::FN, kQuarters = kTileK / 16;
+  static_assert(kQuarters == 4 && kReads <= 2 * kProducts, "");
+  auto read = [&](const uint16_t *buf, int kk, int r) {
+    if (r < S::FN) fb[kk & 1][r] = OpB::read(buf + S::BM * kTileK, wn * S::TN + r * 32, kk, lane);
+    else fa[kk & 1][r - S::FN] = OpA::read(buf, wm * S::TM + (r - S::FN) * 32, kk, lane);
+  };
+  // Quarter kk's products; between them the reads of quarter `then` and loads from..to - 1.
+  auto quarter = [&](int kk, const uint16_t *from, int then, uint16_t *into, int first, int last) {
+#pragma unroll
+    for (int p = 0; p < kProducts; ++p) {
+#pragma unroll
+      for (int r = p * 2; r < p * 2 + 2; ++r)
+        if (r < kReads) read(from, then, r);
+#pragma unroll
+      for (int l = 0; l < kLoads; ++l)
+        if (l >= first && l < last && (l - first) * kProducts / (last - first) == p) load(into, l);
+      const int i = p / S::FN, j = p % S::FN;
+      acc[i][j] = mfma<BF>(fb[kk & 1][j], fa[kk & 1][i], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  if (all > 0) {
+    constexpr int kHalf = kLoads / 2, kAhead = (S::stages - 2) * kLoads;
+#pragma unroll
+    for (int p = 0; p < S::stages; ++p) {
+      aim();
+#pragma unroll
+      for (int l = 0; l < kLoads; ++l)
+        if (p + 1 < S::stages || l < kHalf) load(s_buf + p * S::stage_halves, l);
+    }
+    arrived<kAhead + kHalf>();
+#pragma unroll
+    for (int r = 0; r < kReads; ++r) read(s_buf, 0, r);
+    // step t's buffer, the next one's, and the one whose loads are half under way
+    int now = 0, next = S::stages > 1 ? S::stage_halves : 0, last = (S::stages - 1) * S::stage_halves;
+    for (int t = 0; t < all; ++t) {  // behind the last step zeros are loaded, and not multiplied
+      quarter(0, s_buf + now, 1, s_buf + last, kHalf, kLoads);
+      quarter(1, s_buf + now, 2, nullptr, 0, 0);
+      quarter(2, s_buf + now, 3, nullptr, 0, 0);
+      arrived<kAhead>();
+      aim();
+      quarter(3, s_buf + next, 0, s_buf + now, 0, kHalf);
+      last = now;
+      now = next;
+      next = next + S::stage_halves == S::stages * S::stage_halves ? 0 : next + S::stage_halves;
+    }
+  }
+
+  arrived<0>();  // the buffers are free: nothing is on its way into them
+  if (size.splits > 1) {  // a lane's sums as they are, one line a wave and register
+    float4v *to = reinterpret_cast<float4v *>(size.partial + ((int64_t)tile_number<SYM>(size, z, ti, tj) * size.splits + share) * (S::BM * S::BN) +
+                                              wave * S::wave_sums) + lane;
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < S::FN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float16v &f = acc[i][j];
+          to[((i * S::FN + j) * 4 + q) * 64] = float4v{f[q * 4], f[q * 4 + 1], f[q * 4 + 2], f[q * 4 + 3]};
+        }
+    return;
+  }
+  finish<S>(epilogue, z, ti * S::BM + wm * S::TM, tj * S::BN + wn * S::TN, acc, SYM && ti != tj, s_buf + wave * epilogue_halves<S>(), lane);
+}
+
+// The sums of a tile's shares, in their order, and what becomes of them: a workgroup of one wave for each wave's part.
+template <class S, bool SYM, class Epilogue>
+__global__ __launch_bounds__(64) void k_join(MatSize size, Epilogue epilogue) {
+  __shared__ __attribute__((aligned(16))) uint16_t s_sums[epilogue_halves<S>()];
+  int z, ti, tj, wave;
+  tile_of<SYM>(size, S::W, wave, z, ti, tj);
+  const int lane = threadIdx.x;
+  const float4v *from = reinterpret_cast<const float4v *>(size.partial + (int64_t)tile_number<SYM>(size, z, ti, tj) * size.splits * (S::BM * S::BN) +
+                                                          wave * S::wave_sums) + lane;
+  float16v acc[S::FM][S::FN];
+#pragma unroll
+  for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) acc[i][j] = float16v{};
+  for (int share = 0; share < size.splits; ++share, from += S::BM * S::BN / 4) {
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < S::FN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float4v f = from[((i * S::FN + j) * 4 + q) * 64];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][q * 4 + e] += f[e];
+        }
+  }
+  finish<S>(epilogue, z, ti * S::BM + wave / S::WN * S::TM, tj * S::BN + wave % S::WN * S::TN, acc, SYM && ti != tj, s_sums, lane);
+}
+
+template <class S, bool AK, bool BK, bool BF, bool SYM, class Epilogue>
+inline int launch_tiles(MatSize size, const MatOperand &a, const MatOperand &b, const Epilogue &e, hipStream_t stream) {
+  static_assert(!SYM || S::BM == S::BN, "a triangle of square tiles");
+  size.tiles_m = (size.m + S::BM - 1) / S::BM;
+  size.tiles_n = (size.n + S::BN - 1) / S::BN;
+  const int64_t tiles = (SYM ? (int64_t)size.tiles_m * (size.tiles_m + 1) / 2 : (int64_t)size.tiles_m * size.tiles_n) * size.batch;
+  if (tiles * (size.splits > S::W ? size.splits : S::W) > 0x7fffffffll) return fail(ZEN_EINVAL, "matrix product: too many tiles");
+  k_tiles<S, AK, BK, BF, SYM, Epilogue><<<dim3((unsigned)(tiles * size.splits)), dim3(S::threads), 0, stream>>>(size, a, b, e);
+  ZEN_LAUNCH_CHECK("k_tiles");
+  if (size.splits > 1) {
+    k_join<S, SYM, Epilogue><<<dim3((unsigned)(tiles * S::W)), dim3(64), 0, stream>>>(size, e);
+    ZEN_LAUNCH_CHECK("k_join");
+  }
+  return ZEN_OK;
+}
+
+// ---------------------------------------------------------------- which tiles
+
+// What a step of 64 k costs a compute unit, in us: measured with products of one to a few rounds of tiles (2048 x 2048 and 4096 x
+// 4096, k 1024 to 4096).  Large tiles read LDS and L2 least for their sums (4096^3: 126 us with 256, 190 us with 128, 309 us with 64);
+// small ones fill the card where there are few (1024 x 1024 x 4096: 85, 37 and 29 us).  A launch costs some us
+// apart from its steps, and so does joining the shares of tiles that are split.
+struct TileCost {
+  int side;
+  int at_once;       // workgroups that a compute unit holds
+  float step, lone;  // us, with that many on every compute unit, or one at most
+  float launch;      // us, with the epilogue
+  bool k_only;       // operands with k contiguous only
+};
+constexpr TileCost kTileCosts[] = {
+    {256, 1, 1.85f, 1.50f, 10.f, false}, {192, 1, 1.20f, 1.00f, 8.f, true},
+    {128, 2, 1.10f, 1.10f, 6.f, false}, {128, 1, 0.66f, 0.45f, 6.f, false}, {64, 2, 0.60f, 0.34f, 4.f, false}};
+constexpr int kMostSplits = 16;
+
+struct TilePlan {
+  int side, at_once, splits;
+  size_t partial_bytes;
+};
+
+inline TilePlan plan_tiles(int64_t m, int64_t n, int64_t k, int parts, int64_t batch, bool sym, bool by_k) {
+  const int64_t steps = ceil_div(k, kTileK) * parts;
+  TilePlan best = {64, 2, 1, 0};
+  double least = 1e30;
+  for (const TileCost &c : kTileCosts) {
+    if (c.k_only && !by_k) continue;
+    const int64_t down = ceil_div(m, c.side), across = ceil_div(n, c.side);
+    const int64_t tiles = (sym ? down * (down + 1) / 2 : down * across) * batch;
+    for (int splits = 1; splits <= kMostSplits && (splits == 1 || (tiles * splits <= 512 && steps / splits >= 4)); ++splits) {
+      const int64_t groups = tiles * splits;
+      const double step = groups <= 256 ? c.lone + (c.step / c.at_once - c.lone) * (c.at_once == 1 ? groups / 256.0 : 0.0) : c.step;
+      const double rounds = groups <= 256 ? 1.0 : (double)ceil_div(groups, 256 * c.at_once);
+      const double bytes = splits > 1 ? 4.0 * groups * c.side * c.side : 0.0;
+      const double us = rounds * (double)ceil_div(steps, splits) * step + c.launch + (splits > 1 ? 5.0 + bytes / 2e6 : 0.0);
+      if (us < least) {
+        least = us;
+        best = {c.side, c.at_once, splits, (size_t)bytes};
+      }
+    }
+  }
+  return best;
+}
+
+using Tile256 = TileShape<256, 256, 2, 4, 2>;
+using Tile192 = TileShape<192, 192, 2, 2, 3>;
+using Tile128 = TileShape<128, 128, 2, 2, 2>;      // two workgroups to a compute unit
+using Tile128Deep = TileShape<128, 128, 2, 2, 4>;  // one: where there are no more, they spread over all units, loads further ahead
+using Tile64 = TileShape<64, 64, 2, 2, 4>;
+
+// The product as planned; partial: plan.partial_bytes.
+template <bool AK, bool BK, bool BF, bool SYM, class Epilogue>
+inline int run_tiles(const TilePlan &plan, float *partial, MatSize size, const MatOperand &a, const MatOperand &b, const Epilogue &e,
+                     hipStream_t stream) {
+  size.splits = plan.splits;
+  size.partial = partial;
+  if (plan.side == 256) return launch_tiles<Tile256, AK, BK, BF, SYM>(size, a, b, e, stream);
+  if constexpr (AK && BK)
+    if (plan.side == 192) return launch_tiles<Tile192, AK, BK, BF, SYM>(size, a, b, e, stream);
+  if (plan.side == 128 && plan.at_once == 1) return launch_tiles<Tile128Deep, AK, BK, BF, SYM>(size, a, b, e, stream);
+  if (plan.side == 128) return launch_tiles<Tile128, AK, BK, BF, SYM>(size, a, b, e, stream);
+  return launch_tiles<Tile64, AK, BK, BF, SYM>(size, a, b, e, stream);
+}
 
 // Matrices laid out for the tiles: `rows` x `cols` values at any strides become 16-bit rows of `ld` elements, zeros beyond
 // `cols` and from `rows` to `rows_all` (zen_pack.hip).  Raw: the 16 bits as they are; else value * scale[matrix], in fp16 and, with
-// `low`, what that rounding left over in fp16 again.
+// `low`, what that rounding left over in fp16 again; with `turned`, its transpose too (rows_all and ld are multiples of 64).
 struct PackArgs {
   MatList in;
   int64_t rs, cs;
   int dtype;
   int rows, cols, rows_all;
   int batch;
-  uint16_t *out, *low;
+  uint16_t *out, *low, *turned, *turned_low;
   int64_t ld, out_batch;
   const double *squares;  // null: raw.  Else `shares` sums of squares a matrix, and scale = unit / (root of their sum + eps)
   int shares;
