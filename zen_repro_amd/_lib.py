@@ -183,12 +183,11 @@ def lib():
         "zen_table_gather": (i32, [vp, i64, i32, vp, i32, i64, vp, vp, i64, vp, sz, vp]),
         "zen_momentum": (i32, [vp, i32, vp, i32, i64, ctypes.c_float, i32, vp, i32, vp]),
         "zen_momentum_lists_workspace": (sz, [i64, i32]),
-        "zen_momentum_lists": (i32, [vp, i32, ctypes.POINTER(vp), i32, ctypes.POINTER(vp), i32, ctypes.POINTER(i64),
-                                     ctypes.POINTER(vp), i32, i64, ctypes.c_float, i32, vp, i32, vp, sz, vp, vp]),
-        "zen_product_workspace": (sz, [ctypes.POINTER(ProductArgs)]),
-        "zen_product": (i32, [ctypes.POINTER(ProductArgs)]),
+        "zen_momentum_lists": (i32, [vp, i32, vp, i32, vp, i32, vp, vp, i32, i64, ctypes.c_float, i32, vp, i32, vp, sz, vp, vp]),
+        "zen_product_workspace": (sz, [vp]),
+        "zen_product": (i32, [vp]),
         "zen_orthogonal_workspace": (sz, [i64, i64, i64, i32]),
-        "zen_orthogonal": (i32, [ctypes.POINTER(OrthogonalArgs)]),
+        "zen_orthogonal": (i32, [vp]),
         "zen_stream_read": (i32, [vp, sz, vp, vp]),
         "zen_profile_enable": (i32, [i32]),
         "zen_profile_only": (i32, [i32]),

@@ -8,8 +8,11 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <array>
+#include <limits>
 #include <map>
 #include <optional>
+#include <string>
 #include <tuple>
 #include <utility>
 #include <vector>
@@ -311,6 +314,343 @@ py::tuple step_buffers(int64_t args, Zeros &zeros, const Tensor &flat, const Ten
   return py::make_tuple(py::make_tuple(idx, val, splits, status), py::make_tuple(m_idx, m_val, count, m_status), wait);
 }
 
+// ------------------------------------------------- update.py: arguments are checked here too, in a microsecond or two
+
+int type_of(const Tensor &t, const char *name, bool half = true, bool single = true) {
+  switch (t.scalar_type()) {
+    case at::kFloat:
+      if (single) return ZEN_F32;
+      break;
+    case at::kBFloat16:
+      return ZEN_BF16;
+    case at::kHalf:
+      if (half) return ZEN_F16;
+      break;
+    default:
+      break;
+  }
+  throw py::type_error(std::string(name) + " must be " + (single ? "float32, " : "") + "bfloat16" + (half ? " or float16" : "") +
+                       ", got " + c10::toString(t.scalar_type()));
+}
+
+void on_one_device(const Tensor &first, const Tensor &t) {
+  if (t.device() != first.device())
+    throw py::value_error("tensors on different devices: " + first.device().str() + " and " + t.device().str());
+}
+
+void on_gpu(const Tensor &t) {
+  if (!t.is_cuda()) throw py::type_error("expected GPU tensors");
+}
+
+void plain(const Tensor &t, const char *name) {
+  if (!t.is_contiguous()) throw std::runtime_error(std::string(name) + " must be contiguous");
+}
+
+void not_differentiated(const Tensor &t) {
+  if (t.requires_grad() && at::GradMode::is_enabled())
+    throw std::runtime_error("an optimiser's step is not differentiated: call this under torch.no_grad()");
+}
+
+void written(const Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// First byte, and the byte behind the last one, of what a tensor's elements cover.
+std::pair<const char *, const char *> extent(const Tensor &t) {
+  if (t.numel() == 0) return {nullptr, nullptr};
+  const char *first = static_cast<const char *>(t.data_ptr());
+  int64_t last = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  return {first, first + (last + 1) * t.element_size()};
+}
+
+// Whether two tensors may share memory.  Told apart beside plain stretches: two equally strided matrices whose rows lie between
+// each other's (column ranges of one larger matrix).
+bool overlap(const Tensor &a, const Tensor &b) {
+  const auto [a0, a1] = extent(a);
+  const auto [b0, b1] = extent(b);
+  if (!(a0 < b1 && b0 < a1)) return false;
+  if (a.dim() == 2 && b.dim() == 2 && a.strides() == b.strides() && a.scalar_type() == b.scalar_type()) {
+    const int line = a.stride(1) == 1 ? 1 : 0;  // the dimension whose neighbours are neighbours in memory
+    const int64_t step = a.stride(1 - line), size = a.element_size(), away = b0 - a0;
+    if (a.stride(line) == 1 && step > 0 && away % size == 0) {
+      const int64_t apart = (away / size % step + step) % step;
+      if (a.size(line) <= apart && apart <= step - b.size(line)) return false;
+    }
+  }
+  return true;
+}
+
+bool same(const Tensor &a, const Tensor &b) {
+  return a.data_ptr() == b.data_ptr() && a.scalar_type() == b.scalar_type() && a.sizes() == b.sizes() && a.strides() == b.strides();
+}
+
+// Refuses a tensor to be written some of whose elements are one place in memory.
+void one_place(const Tensor &t, const char *name) {
+  std::vector<std::pair<int64_t, int64_t>> at;
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1) at.emplace_back(t.stride(d), t.size(d));
+  std::sort(at.begin(), at.end());
+  int64_t reach = 0;
+  for (const auto &[stride, size] : at) {
+    if (stride <= reach) throw py::value_error(std::string(name) + ": several elements are one place in memory");
+    reach += (size - 1) * stride;
+  }
+}
+
+using Dtype = std::optional<at::ScalarType>;
+
+Tensor momentum_out(const Tensor &momentum, double mu, const Dtype &dtype, const std::optional<Tensor> &out, at::ScalarType like) {
+  on_gpu(momentum);
+  type_of(momentum, "momentum", false);
+  plain(momentum, "momentum");
+  not_differentiated(momentum);
+  if (!(mu >= 0.0 && mu < std::numeric_limits<double>::infinity())) throw py::value_error("mu must be finite and not negative");
+  if (!out) return made([&] { return at::empty(momentum.sizes(), momentum.options().dtype(dtype ? *dtype : like).requires_grad(false)); });
+  if (dtype && out->scalar_type() != *dtype) throw py::type_error("out is not of that dtype");
+  on_one_device(momentum, *out);
+  not_differentiated(*out);
+  plain(*out, "out");
+  if (out->sizes() != momentum.sizes()) throw py::value_error("out is not of the momentum's shape");
+  if (overlap(*out, momentum)) throw py::value_error("out overlaps the momentum");
+  return *out;
+}
+
+py::tuple momentum(const py::object &fn, const Tensor &momentum, const Tensor &grad, double mu, bool nesterov, const Dtype &dtype,
+                   const std::optional<Tensor> &given, int64_t stream) {
+  on_gpu(grad);
+  const int code = type_of(grad, "grad");
+  const Tensor out = momentum_out(momentum, mu, dtype, given, grad.scalar_type());
+  const int out_code = type_of(out, "update");
+  on_one_device(momentum, grad);
+  plain(grad, "grad");
+  not_differentiated(grad);
+  if (grad.sizes() != momentum.sizes()) throw py::value_error("grad is not of the momentum's shape");
+  if (overlap(grad, momentum) || (overlap(out, grad) && !same(out, grad)))
+    throw py::value_error("grad overlaps the momentum or a part of out");
+  const py::object rc = fn(address(momentum), type_of(momentum, "momentum"), address(grad), code, grad.numel(), mu, nesterov ? 1 : 0,
+                           address(out), out_code, stream);
+  written(momentum);
+  written(out);
+  return py::make_tuple(rc, out);
+}
+
+// counts: none, one tensor (an element to a list), or one tensor or none to a list
+py::tuple momentum_lists(const py::object &fn, Zeros &zeros, const Tensor &momentum, const std::vector<Tensor> &indices,
+                         const std::vector<Tensor> &values, double mu, bool nesterov, const std::optional<Tensor> &counted,
+                         const std::optional<std::vector<std::optional<Tensor>>> &counts, const Dtype &dtype,
+                         const std::optional<Tensor> &given, const py::object &workspace, int64_t stream) {
+  const size_t lists = indices.size();
+  if (lists < 1 || lists > ZEN_MOMENTUM_LISTS_MOST || values.size() != lists)
+    throw py::value_error("1 to " + std::to_string(ZEN_MOMENTUM_LISTS_MOST) + " lists, as many of indices as of values: got " +
+                          std::to_string(lists) + " and " + std::to_string(values.size()));
+  on_gpu(values[0]);
+  const int code = type_of(values[0], "values");
+  const at::ScalarType index = indices[0].scalar_type();
+  if (index != at::kInt && index != at::kLong) throw py::type_error("indices must be int32 or int64");
+  const Tensor out = momentum_out(momentum, mu, dtype, given, values[0].scalar_type());
+  const int out_code = type_of(out, "update");
+  const int64_t n = momentum.numel();
+  if (n > 0x7fffffffll) throw py::value_error("momentum_update_sparse: at most 2^31 - 1 elements");
+  const auto apart = [&](const Tensor &t) {
+    if (overlap(t, momentum) || overlap(t, out)) throw py::value_error("momentum_update_sparse: a list overlaps the momentum or out");
+  };
+  for (size_t l = 0; l < lists; ++l) {
+    const Tensor &i = indices[l], &v = values[l];
+    on_one_device(momentum, i);
+    on_one_device(momentum, v);
+    plain(i, "indices");
+    plain(v, "values");
+    not_differentiated(v);
+    if (i.scalar_type() != index || v.scalar_type() != values[0].scalar_type())
+      throw py::type_error("the lists' indices, and their values, have one type");
+    if (i.numel() != v.numel()) throw py::value_error("a list has as many indices as values");
+    if (n == 0 && i.numel()) throw py::value_error("momentum_update_sparse: entries for an empty momentum");
+    apart(i);
+    apart(v);
+  }
+  std::vector<int64_t> count(lists, 0);
+  const auto check = [&](const Tensor &c, int64_t elements) {
+    on_one_device(momentum, c);
+    if (c.scalar_type() != at::kLong) throw py::type_error("counts are int64");
+    if (c.numel() != elements || c.dim() > 1) throw py::value_error("counts: one element to a list");
+    apart(c);
+  };
+  if (counted) {
+    check(*counted, (int64_t)lists);
+    for (size_t l = 0; l < lists; ++l) count[l] = address(*counted) + 8 * (int64_t)l * (counted->dim() ? counted->stride(0) : 0);
+  } else if (counts) {
+    if (counts->size() != lists) throw py::value_error("counts: one to a list");
+    for (size_t l = 0; l < lists; ++l)
+      if ((*counts)[l]) {
+        check(*(*counts)[l], 1);
+        count[l] = address(*(*counts)[l]);
+      }
+  }
+  const Tensor status = made([&] { return zeros.status(momentum, stream); });
+  const Lists i(indices), v(values);
+  const py::object rc = fn(address(momentum), type_of(momentum, "momentum"), i.addresses(), index == at::kLong ? 1 : 0, v.addresses(),
+                           code, i.counts(), reinterpret_cast<int64_t>(count.data()), lists, n, mu, nesterov ? 1 : 0, address(out),
+                           out_code, workspace.is_none() ? 0 : address(workspace.cast<Tensor>()),
+                           workspace.is_none() ? 0 : workspace.cast<Tensor>().numel(), address(status), stream);
+  written(momentum);
+  written(out);
+  return py::make_tuple(rc, out, status);
+}
+
+// `room(bytes)` gives a workspace.
+py::tuple product(const py::object &fn, const py::object &bytes_of, const py::object &room, const Tensor &a, const Tensor &b,
+                  const std::optional<Tensor> &residual, double alpha, double beta, bool symmetric, const Dtype &dtype,
+                  const std::optional<Tensor> &given, int64_t stream) {
+  on_gpu(a);
+  zen_product_args p = {};
+  p.dtype = type_of(a, "a", true, false);
+  on_one_device(a, b);
+  not_differentiated(a);
+  not_differentiated(b);
+  if (b.scalar_type() != a.scalar_type()) throw py::type_error("a and b are not of one type");
+  const int64_t d = a.dim();
+  if ((d != 2 && d != 3) || b.dim() != d) throw py::value_error("a and b are two matrices, or two stacks of matrices");
+  p.batch = d == 3 ? a.size(0) : 1;
+  p.m = a.size(-2);
+  p.k = a.size(-1);
+  p.n = b.size(-1);
+  if (b.size(-2) != p.k || (d == 3 && b.size(0) != p.batch)) throw py::value_error("these shapes have no product");
+  if (symmetric && p.m != p.n) throw py::value_error("a symmetric result is square");
+  std::vector<int64_t> shape = {p.m, p.n};
+  if (d == 3) shape.insert(shape.begin(), p.batch);
+  if (residual) {
+    on_one_device(a, *residual);
+    not_differentiated(*residual);
+    if (residual->sizes() != at::IntArrayRef(shape)) throw py::value_error("residual is not of the product's shape");
+    p.c = residual->data_ptr();
+    p.c_dtype = type_of(*residual, "residual");
+    p.c_rs = residual->stride(-2);
+    p.c_cs = residual->stride(-1);
+    p.c_batch = d == 3 ? residual->stride(0) : 0;
+  }
+  const Tensor out = given ? *given : made([&] {
+    return at::empty(shape, a.options().dtype(dtype ? *dtype : residual ? residual->scalar_type() : a.scalar_type()).requires_grad(false));
+  });
+  if (given) {
+    on_one_device(a, out);
+    not_differentiated(out);
+    if (out.sizes() != at::IntArrayRef(shape)) throw py::value_error("out is not of the product's shape");
+    if (dtype && out.scalar_type() != *dtype) throw py::type_error("out is not of that dtype");
+    one_place(out, "out");
+    if (overlap(out, a) || overlap(out, b) || (residual && overlap(out, *residual) && !same(out, *residual)))
+      throw py::value_error("out overlaps an input");
+  }
+  p.out_dtype = type_of(out, "the result");
+  p.a = a.data_ptr();
+  p.a_rs = a.stride(-2);
+  p.a_cs = a.stride(-1);
+  p.b = b.data_ptr();
+  p.b_rs = b.stride(-2);
+  p.b_cs = b.stride(-1);
+  p.out = out.data_ptr();
+  p.out_rs = out.stride(-2);
+  p.out_cs = out.stride(-1);
+  if (d == 3) {
+    p.a_batch = a.stride(0);
+    p.b_batch = b.stride(0);
+    p.out_batch = out.stride(0);
+  }
+  p.alpha = (float)alpha;
+  p.beta = (float)beta;
+  p.symmetric = symmetric;
+  p.stream = reinterpret_cast<void *>(stream);
+  const int64_t args = reinterpret_cast<int64_t>(&p);
+  p.workspace_bytes = bytes_of(args).cast<size_t>();
+  Tensor ws;
+  if (p.workspace_bytes) {
+    ws = room(p.workspace_bytes).cast<Tensor>();
+    p.workspace = ws.data_ptr();
+  }
+  const py::object rc = fn(args);
+  written(out);
+  return py::make_tuple(rc, out);
+}
+
+// Updates to outs (or weights), one zen_orthogonal call for each pair of strides among them; its first failure, or 0.
+py::object orthogonal(const py::object &fn, const py::object &bytes_of, const py::object &room, const std::string &what,
+                      const std::vector<Tensor> &updates, const std::vector<Tensor> &outs, int steps, double a, double b, double c,
+                      double eps, bool precise, bool weights, double keep, double gain, int64_t stream) {
+  const Tensor &first = updates[0];
+  on_gpu(first);
+  if (steps < 1) throw py::value_error(what + ": at least one step");
+  if (!(eps >= 0)) throw py::value_error(what + ": eps must not be negative");
+  zen_orthogonal_args p = {};
+  p.update_dtype = type_of(first, "update");
+  p.out_dtype = type_of(outs[0], weights ? "weight" : "out");
+  std::map<std::array<int64_t, 4>, std::pair<std::vector<int64_t>, std::vector<int64_t>>> groups;
+  struct Span {
+    const char *from, *to;
+    bool writes;
+    const Tensor *t;
+  };
+  std::vector<Span> spans;
+  for (size_t i = 0; i < updates.size(); ++i) {
+    const Tensor &u = updates[i], &o = outs[i];
+    on_one_device(first, u);
+    on_one_device(first, o);
+    not_differentiated(u);
+    not_differentiated(o);
+    if (u.sizes() != first.sizes() || u.scalar_type() != first.scalar_type() || o.scalar_type() != outs[0].scalar_type())
+      throw py::value_error(what + ": the matrices of a call have one shape and one type");
+    if (o.sizes() != u.sizes()) throw py::value_error(what + ": an update and its result are of different shapes");
+    one_place(o, what.c_str());
+    const auto eo = extent(o);
+    spans.push_back({eo.first, eo.second, true, &o});
+    if (weights || !same(u, o)) {
+      const auto eu = extent(u);
+      spans.push_back({eu.first, eu.second, false, &u});
+    }
+    auto &g = groups[{u.stride(0), u.stride(1), o.stride(0), o.stride(1)}];
+    g.first.push_back(address(u));
+    g.second.push_back(address(o));
+  }
+  if (first.numel() == 0) return py::int_(0);
+  // what is written lies apart from everything else (an update may be its own result)
+  std::sort(spans.begin(), spans.end(), [](const Span &x, const Span &y) { return x.from < y.from; });
+  std::vector<const Span *> open;
+  for (const Span &s : spans) {
+    open.erase(std::remove_if(open.begin(), open.end(), [&](const Span *o) { return o->to <= s.from; }), open.end());
+    for (const Span *o : open)
+      if ((s.writes || o->writes) && overlap(*s.t, *o->t)) throw py::value_error(what + ": a result overlaps another matrix");
+    open.push_back(&s);
+  }
+  p.rows = first.size(0);
+  p.cols = first.size(1);
+  p.steps = steps;
+  p.a = (float)a;
+  p.b = (float)b;
+  p.c = (float)c;
+  p.eps = eps;
+  p.precise = precise;
+  p.weights = weights;
+  p.keep = (float)keep;
+  p.gain = (float)gain;
+  p.stream = reinterpret_cast<void *>(stream);
+  py::object rc = py::int_(0);
+  for (auto &[strides, g] : groups) {
+    p.count = (int64_t)g.first.size();
+    p.updates = reinterpret_cast<const void *const *>(g.first.data());
+    p.outs = reinterpret_cast<void *const *>(g.second.data());
+    p.update_rs = strides[0];
+    p.update_cs = strides[1];
+    p.out_rs = strides[2];
+    p.out_cs = strides[3];
+    p.workspace_bytes = bytes_of(p.rows, p.cols, p.count, precise ? 1 : 0).cast<size_t>();
+    const Tensor ws = room(p.workspace_bytes).cast<Tensor>();
+    p.workspace = ws.data_ptr();
+    rc = fn(reinterpret_cast<int64_t>(&p));
+    if (rc.cast<int>() != ZEN_OK) break;
+  }
+  for (const Tensor &o : outs) written(o);
+  return rc;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -332,4 +672,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("table_find", &table_find);
   m.def("table_gather", &table_gather);
   m.def("step_buffers", &step_buffers);
+  m.def("momentum", &momentum);
+  m.def("momentum_lists", &momentum_lists);
+  m.def("product", &product);
+  m.def("orthogonal", &orthogonal);
 }
