@@ -20,31 +20,116 @@ namespace {
 
 constexpr float kUnit = 1024.f;
 constexpr int kSquareBlock = 256;
-constexpr int kMostShares = 256;  // workgroups to a matrix' sum of squares
+constexpr int kMostShares = 1024;  // workgroups to a matrix' sum of squares
 
 
-// Sums of squares in fp64 (an fp32 square overflows from 2^64 on), one a workgroup, in a fixed order.
-__global__ __launch_bounds__(kSquareBlock) void k_squares(MatList in, int64_t rs, int64_t cs, int dtype, int rows, int cols,
-                                                          int shares, double *__restrict__ sums) {
+// Sums of squares in fp64 (an fp32 square overflows from 2^64 on), one a workgroup, in a fixed order.  `slow` lines of `fast`
+// values; wide: a line is contiguous and begins at a multiple of 16 bytes.  Bound by the read.
+__global__ __launch_bounds__(kSquareBlock) void k_squares(MatList in, int64_t slow_stride, int64_t fast_stride, int dtype, int slow,
+                                                          int fast, int wide, int shares, double *__restrict__ sums) {
   __shared__ double s_sum[kSquareBlock / 64];
   const int share = blockIdx.x, z = blockIdx.y;
   const char *p = in.of(z);
-  const int64_t slow = cs <= rs ? rows : cols, fast = cs <= rs ? cols : rows;
-  const int64_t slow_stride = cs <= rs ? rs : cs, fast_stride = cs <= rs ? cs : rs;
-  double sum = 0.0;
-  for (int64_t i = share; i < slow; i += shares)
-    for (int64_t j = threadIdx.x; j < fast; j += kSquareBlock) {
-      const double v = (double)load_value(p, i * slow_stride + j * fast_stride, dtype);
-      sum = fma(v, v, sum);
+  const int64_t pieces = (fast + 7) / 8, all = pieces * slow;
+  const int64_t first = all * share / shares, last = all * (share + 1) / shares;
+  double even = 0.0, odd = 0.0;
+#pragma unroll 2
+  for (int64_t at = first + threadIdx.x; at < last; at += kSquareBlock) {
+    const int64_t i = at / pieces;
+    const int j = (int)(at - i * pieces) * 8;
+    if (wide && j + 8 <= fast) {
+      const float8v v = load_eight(p, i * slow_stride + j, dtype);
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        even = fma((double)v[e], (double)v[e], even);
+        odd = fma((double)v[e + 1], (double)v[e + 1], odd);
+      }
+    } else {
+      for (int e = j; e < j + 8 && e < fast; ++e) {
+        const double v = (double)load_value(p, i * slow_stride + e * fast_stride, dtype);
+        even = fma(v, v, even);
+      }
     }
+  }
+  double sum = even + odd;
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
   if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
-    double all = 0.0;
-    for (int w = 0; w < kSquareBlock / 64; ++w) all += s_sum[w];
-    sums[(int64_t)z * shares + share] = all;
+    double all_waves = 0.0;
+    for (int w = 0; w < kSquareBlock / 64; ++w) all_waves += s_sum[w];
+    sums[(int64_t)z * shares + share] = all_waves;
+  }
+}
+
+constexpr int kLaySide = 64;
+
+// X = U / (|U| + eps) and its transpose, in fp16 and what that leaves over, in whole steps of the products with zeros behind the
+// matrix' own (fp64: a tiny update's scale is beyond fp32).  A workgroup takes 64 lines of 64 neighbours: one of the two goes out as
+// it was read, the other through LDS.  Bound by memory: one read, three or four writes.
+struct LayOut {
+  MatList in;
+  int64_t slow_stride, fast_stride;
+  int dtype, slow, fast, wide;
+  _Float16 *along, *along_low;  // lines as they lie in memory, of along_ld; null low: not kept
+  _Float16 *across, *across_low;
+  int64_t along_ld, across_ld, batch;
+  const double *squares;
+  int shares;
+  double eps;
+};
+
+__device__ __forceinline__ void put_halves(_Float16 *hi, _Float16 *low, int64_t at, float8v v) {
+  const half8v h = __builtin_convertvector(v, half8v);
+  *reinterpret_cast<half8v *>(hi + at) = h;
+  if (low) *reinterpret_cast<half8v *>(low + at) = __builtin_convertvector(v - widen(h), half8v);
+}
+
+__global__ __launch_bounds__(256) void k_lay_out(LayOut p) {
+  __shared__ float s_tile[kLaySide][kLaySide + 1];
+  __shared__ double s_sum[4];
+  const int z = blockIdx.z, f0 = blockIdx.x * kLaySide, s0 = blockIdx.y * kLaySide, tid = threadIdx.x;
+  const char *in = p.in.of(z);
+  float8v v[2];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int s = s0 + q * 32 + tid / 8, f = f0 + tid % 8 * 8;
+    v[q] = float8v{};
+    if (s < p.slow && p.wide && f + 8 <= p.fast) {
+      v[q] = load_eight(in, s * p.slow_stride + f, p.dtype);
+    } else if (s < p.slow) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (f + e < p.fast) v[q][e] = load_value(in, s * p.slow_stride + (f + e) * p.fast_stride, p.dtype);
+    }
+  }
+  double sum = 0.0;
+  for (int i = tid; i < p.shares; i += 256) sum += p.squares[(int64_t)z * p.shares + i];
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+  if ((tid & 63) == 0) s_sum[tid >> 6] = sum;
+  __syncthreads();
+  const double norm = sqrt((s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3])) + p.eps;
+  const double scale = norm == 0.0 ? 0.0 : (double)kUnit / norm;  // nothing but zeros, and eps is zero
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int s = q * 32 + tid / 8, f = tid % 8 * 8;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[q][e] = (float)((double)v[q][e] * scale);
+      s_tile[s][f + e] = v[q][e];
+    }
+    put_halves(p.along, p.along_low, z * p.batch + (s0 + s) * p.along_ld + f0 + f, v[q]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int f = q * 32 + tid / 8, s = tid % 8 * 8;
+    float8v w;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = s_tile[s + e][f];
+    put_halves(p.across, p.across_low, z * p.batch + (f0 + f) * p.across_ld + s0 + s, w);
   }
 }
 
@@ -63,9 +148,8 @@ struct Room {
 };
 
 int shares_of(int64_t rows, int64_t cols) {
-  const int64_t want = rows * cols / 8192 + 1, slow = rows > cols ? rows : cols;
-  const int64_t most = want < kMostShares ? want : kMostShares;
-  return (int)(most < slow ? most : slow);
+  const int64_t want = rows * cols / 4096 + 1;
+  return (int)(want < kMostShares ? want : kMostShares);
 }
 
 int chunk_of(int64_t m, int64_t n, int64_t count) {
@@ -123,29 +207,26 @@ int chunk(const zen_orthogonal_args &p, const Room &r, int64_t first, int batch,
     out.at[i] = static_cast<char *>(p.outs[first + i]);
   }
   const int64_t rs = turn ? p.update_cs : p.update_rs, cs = turn ? p.update_rs : p.update_cs;
-  k_squares<<<dim3((unsigned)shares, (unsigned)batch), dim3(kSquareBlock), 0, s>>>(in, rs, cs, p.update_dtype, small, large,
-                                                                                 shares, r.squares);
+  const bool across = cs <= rs;  // memory goes along X's rows
+  const int slow = across ? small : large, fast = across ? large : small;
+  const int64_t slow_stride = across ? rs : cs, fast_stride = across ? cs : rs;
+  int wide = fast_stride == 1 && slow_stride * (p.update_dtype == ZEN_F32 ? 4 : 2) % 16 == 0;
+  for (int i = 0; i < batch; ++i) wide &= (reinterpret_cast<uintptr_t>(in.at[i]) & 15u) == 0;
+  k_squares<<<dim3((unsigned)shares, (unsigned)batch), dim3(kSquareBlock), 0, s>>>(in, slow_stride, fast_stride, p.update_dtype, slow,
+                                                                                  fast, wide, shares, r.squares);
   ZEN_LAUNCH_CHECK("k_squares");
-  PackArgs pack = {};
-  pack.in = in;
-  pack.rs = rs;
-  pack.cs = cs;
-  pack.dtype = p.update_dtype;
-  pack.rows = small;
-  pack.cols = large;
-  pack.rows_all = (int)r.m;
-  pack.batch = batch;
-  pack.out = reinterpret_cast<uint16_t *>(r.x);
-  pack.low = reinterpret_cast<uint16_t *>(r.x_low);
-  pack.turned = reinterpret_cast<uint16_t *>(r.turned[0]);
-  pack.turned_low = reinterpret_cast<uint16_t *>(r.turned_low[0]);
-  pack.ld = r.n;
-  pack.out_batch = r.m * r.n;
-  pack.squares = r.squares;
-  pack.shares = shares;
-  pack.eps = p.eps;
-  pack.unit = kUnit;
-  if (const int rc = pack_matrices(pack, s)) return rc;
+  LayOut lay = {in, slow_stride, fast_stride, p.update_dtype, slow, fast, wide, r.x, r.x_low, r.turned[0], r.turned_low[0],
+                r.n, r.m, r.m * r.n, r.squares, shares, p.eps};
+  if (!across) {
+    lay.along = r.turned[0];
+    lay.along_low = r.turned_low[0];
+    lay.along_ld = r.m;
+    lay.across = r.x;
+    lay.across_low = r.x_low;
+    lay.across_ld = r.n;
+  }
+  k_lay_out<<<dim3((unsigned)(lay.along_ld / kLaySide), (unsigned)(lay.across_ld / kLaySide), (unsigned)batch), dim3(256), 0, s>>>(lay);
+  ZEN_LAUNCH_CHECK("k_lay_out");
 
   const int parts = p.precise ? 3 : 1;
   const int m = (int)r.m, n = (int)r.n;

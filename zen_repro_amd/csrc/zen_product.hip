@@ -35,7 +35,7 @@ size_t room(const Side &s, int64_t batches) {
   return s.packed ? align_up((size_t)s.rows * s.ld * batches * 2, 256) : 0;
 }
 
-int lay_out(Side &s, int dtype, int64_t batches, Carver &cv, hipStream_t stream) {
+int lay_out(Side &s, int64_t batches, Carver &cv, hipStream_t stream) {
   if (!s.packed) return ZEN_OK;
   uint16_t *to = cv.take<uint16_t>((size_t)s.rows * s.ld * batches);
   PackArgs p = {};
@@ -43,8 +43,7 @@ int lay_out(Side &s, int dtype, int64_t batches, Carver &cv, hipStream_t stream)
   p.in.stride = s.batch * 2;
   p.rs = s.row;
   p.cs = s.along;
-  p.dtype = dtype;
-  p.rows = p.rows_all = (int)s.rows;
+  p.rows = (int)s.rows;
   p.cols = (int)s.k;
   p.batch = (int)batches;
   p.out = to;
@@ -115,8 +114,8 @@ int zen_product(const zen_product_args *p) {
   const TilePlan how = plan(*p, sa, sb);
   Carver cv(p->workspace);
   if (p->k > 0) {
-    if (const int rc = lay_out(sa, p->dtype, p->batch, cv, s)) return rc;
-    if (const int rc = lay_out(sb, p->dtype, p->batch, cv, s)) return rc;
+    if (const int rc = lay_out(sa, p->batch, cv, s)) return rc;
+    if (const int rc = lay_out(sb, p->batch, cv, s)) return rc;
   }
   const MatSize size = {(int)p->m, (int)p->n, (int)p->k, 0, 0, (int)p->batch, 1, 1, nullptr};
   float *partial = reinterpret_cast<float *>(cv.base + cv.used);

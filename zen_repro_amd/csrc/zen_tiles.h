@@ -642,21 +642,15 @@ inline int run_tiles(const TilePlan &plan, float *partial, MatSize size, const M
   return launch_tiles<Tile64, AK, BK, BF, SYM>(size, a, b, e, stream);
 }
 
-// Matrices laid out for the tiles: `rows` x `cols` values at any strides become 16-bit rows of `ld` elements, zeros beyond
-// `cols` and from `rows` to `rows_all` (zen_pack.hip).  Raw: the 16 bits as they are; else value * scale[matrix], in fp16 and, with
-// `low`, what that rounding left over in fp16 again; with `turned`, its transpose too (rows_all and ld are multiples of 64).
+// Matrices of 16-bit values laid out for the tiles: `rows` x `cols` at any strides become rows of `ld` elements, zeros beyond `cols`
+// (zen_pack.hip).
 struct PackArgs {
   MatList in;
   int64_t rs, cs;
-  int dtype;
-  int rows, cols, rows_all;
+  int rows, cols;
   int batch;
-  uint16_t *out, *low, *turned, *turned_low;
+  uint16_t *out;
   int64_t ld, out_batch;
-  const double *squares;  // null: raw.  Else `shares` sums of squares a matrix, and scale = unit / (root of their sum + eps)
-  int shares;
-  double eps;
-  float unit;
 };
 int pack_matrices(const PackArgs &args, hipStream_t stream);
 
