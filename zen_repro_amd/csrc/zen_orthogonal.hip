@@ -285,8 +285,10 @@ int chunk(const zen_orthogonal_args &p, const Room &r, int64_t first, int batch,
     o.out_rs = turn ? p.out_cs : p.out_rs;
     o.out_cs = turn ? p.out_rs : p.out_cs;
     o.out_type = p.out_dtype;
-    o.lines = o.out_cs == 1 && o.out_rs * (p.out_dtype == ZEN_F32 ? 4 : 2) % 16 == 0;
-    for (int i = 0; i < batch; ++i) o.lines &= (reinterpret_cast<uintptr_t>(out.at[i]) & 15u) == 0;
+    const int64_t size = p.out_dtype == ZEN_F32 ? 4 : 2;
+    o.lines = o.out_cs == 1 && o.out_rs * size % 16 == 0 ? 1 : o.out_rs == 1 && o.out_cs * size % 16 == 0 ? 2 : 0;
+    for (int i = 0; i < batch; ++i)
+      if (reinterpret_cast<uintptr_t>(out.at[i]) & 15u) o.lines = 0;
     o.res.listed = -1;
     if (p.weights) {
       o.res = o.out;

@@ -65,9 +65,10 @@ int go(const TilePlan &plan, float *partial, const MatSize &size, const MatOpera
   return sym ? run_tiles<AK, BK, false, true>(plan, partial, size, a, b, e, s) : run_tiles<AK, BK, false, false>(plan, partial, size, a, b, e, s);
 }
 
-int lines(const void *p, int64_t rs, int64_t cs, int64_t batch, int type, int64_t batches) {
+int lines(const void *p, int64_t rs, int64_t cs, int64_t batch, int type, int64_t batches, bool symmetric) {
   const int64_t size = size_of(type);
-  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && cs == 1 && rs * size % 16 == 0 && (batches <= 1 || batch * size % 16 == 0);
+  if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0 || (batches > 1 && batch * size % 16 != 0)) return 0;
+  return cs == 1 && rs * size % 16 == 0 ? 1 : rs == 1 && cs * size % 16 == 0 && !symmetric ? 2 : 0;
 }
 
 int check(const zen_product_args *p) {
@@ -121,6 +122,7 @@ int zen_product(const zen_product_args *p) {
   float *partial = reinterpret_cast<float *>(cv.base + cv.used);
   const uint16_t *pa = static_cast<const uint16_t *>(sa.p), *pb = static_cast<const uint16_t *>(sb.p);
   const MatOperand a = {{pa, pa}, sa.ld, sa.batch}, b = {{pb, pb}, sb.ld, sb.batch};
+  const bool bf = p->dtype == ZEN_BF16, sym = p->symmetric != 0;
   OutEpilogue e = {};
   e.alpha = p->alpha;
   e.gain = 1.f;
@@ -132,10 +134,10 @@ int zen_product(const zen_product_args *p) {
   e.out_rs = p->out_rs;
   e.out_cs = p->out_cs;
   e.out_type = p->out_dtype;
-  e.lines = lines(p->out, p->out_rs, p->out_cs, p->out_batch, p->out_dtype, p->batch);
+  e.lines = lines(p->out, p->out_rs, p->out_cs, p->out_batch, p->out_dtype, p->batch, sym);
   e.res.listed = -1;
   if (p->c) {
-    e.lines &= lines(p->c, p->c_rs, p->c_cs, p->c_batch, p->c_dtype, p->batch);
+    if (lines(p->c, p->c_rs, p->c_cs, p->c_batch, p->c_dtype, p->batch, sym) != e.lines) e.lines = 0;
     e.res.listed = 0;
     e.res.base = static_cast<char *>(const_cast<void *>(p->c));
     e.res.stride = p->c_batch * size_of(p->c_dtype);
@@ -143,7 +145,6 @@ int zen_product(const zen_product_args *p) {
     e.res_cs = p->c_cs;
     e.res_type = p->c_dtype;
   }
-  const bool bf = p->dtype == ZEN_BF16, sym = p->symmetric != 0;
   if (sa.contiguous)
     return sb.contiguous ? go<true, true>(how, partial, size, a, b, e, bf, sym, s) : go<true, false>(how, partial, size, a, b, e, bf, sym, s);
   return sb.contiguous ? go<false, true>(how, partial, size, a, b, e, bf, sym, s) : go<false, false>(how, partial, size, a, b, e, bf, sym, s);

@@ -67,6 +67,7 @@ struct TileShape {
   static constexpr int stages = STAGES;                              // buffers that go round
   static constexpr int stage_halves = (BM + BN) * kTileK;
   static constexpr int wave_sums = TM * TN;
+  static constexpr bool whole_steps = FM * FN <= 4;                  // read a step ahead, not a quarter
 };
 
 #define ZEN_LDS __attribute__((address_space(3)))
@@ -79,12 +80,12 @@ struct TileOperand {
   static constexpr int row_lanes = KC ? 8 : R / 8;    // lanes to a row of the piece
   static constexpr int rows = 64 / row_lanes;         // rows to a load
   static_assert(KC || (W * rows) % 4 == 0, "the swizzle is the same in every load of a wave");
-  const char *first[2];  // of the tile in the matrix, and in what its rounding left over
-  int64_t all;           // bytes of the operand from there on
-  int64_t step;          // bytes from step to step
-  uint32_t voffset, soffset, vnow;
+  const char *first[2];   // of the tile in the matrix, and in what its rounding left over
+  const char *base;       // of the step that is aimed at next
+  int64_t step;           // bytes from step to step
+  uint32_t records, full, tail;  // bytes there are from `base` on; in the first step; (k as the stride) in the last one
+  uint32_t voffset, vlast, vnow, soffset;
   __amdgpu_buffer_rsrc_t source;
-  int tail_chunk;        // KC: this lane's first k within the step
 
   // k contiguous: piece c of row r lies in place c ^ key(r)
   static __device__ __forceinline__ int key(int r) { return ((r >> 1) & 3) | ((r >> 2) & 4); }
@@ -92,7 +93,8 @@ struct TileOperand {
   // k as the stride: where piece `chunk` of row k of the step lies
   static __device__ __forceinline__ int place(int k, int chunk) { return chunk ^ (R >= 128 ? (k & 3) << 2 : (k & 2) << 1); }
 
-  // r0: first row (i or j) of the tile; rows_all: rows there are; k: the operand's k
+  // r0: first row (i or j) of the tile; rows_all: rows there are; k: the operand's k.  What a step reaches lies within 2^30
+  // bytes (kMostLd), so 32 bits do for everything but the addresses.
   __device__ __forceinline__ void start(const MatOperand &o, int z, int64_t r0, int64_t rows_all, int k, int wave, int lane) {
     const int row = wave * rows + lane / row_lanes;
     const int slot = lane % row_lanes;
@@ -100,21 +102,42 @@ struct TileOperand {
     const int64_t ld = o.ld, from = z * o.batch + (KC ? r0 * ld : r0);
     first[0] = reinterpret_cast<const char *>(o.p[0] + from);
     first[1] = reinterpret_cast<const char *>(o.p[1] + from);
-    tail_chunk = chunk * 8;
-    voffset = (uint32_t)((row * ld + chunk * 8) * 2);
-    // whole pieces: k is a multiple of 8, or ld has room; whole words: the address is a multiple of 16
-    all = KC ? ((rows_all - r0 - 1) * ld + ((k + 7) & ~7)) * 2 : (((int64_t)k - 1) * ld + ((rows_all - r0 + 1) & ~1ll)) * 2;
-    step = KC ? kTileK * 2 : kTileK * ld * 2;
+    const int rest = (k - 1) % kTileK + 1;  // k of the last step
+    voffset = vlast = (uint32_t)((row * ld + chunk * 8) * 2);
+    if (KC) {
+      const int64_t lines = rows_all - r0 < R ? rows_all - r0 : R;
+      full = (uint32_t)(((lines - 1) * ld + ((k + 7) & ~7)) * 2);  // whole pieces: k is a multiple of 8, or ld has room
+      tail = 0;
+      step = kTileK * 2;
+      if (chunk * 8 >= rest) vlast = 0x80000000u;
+    } else {
+      const int64_t line = (rows_all - r0 + 1) & ~1ll;  // whole words: the address is a multiple of 16
+      const int64_t most = line < ld ? line : ld;
+      full = (uint32_t)(((kTileK - 1) * ld + most) * 2);
+      tail = (uint32_t)(((rest - 1) * ld + most) * 2);
+      step = kTileK * ld * 2;
+    }
     soffset = (uint32_t)(W * rows * ld * 2);
   }
 
-  // What the loads of step `at` (of `low`'s matrix) read: nothing where `there` is false (zeros arrive).
-  __device__ __forceinline__ void aim(int at, bool low, bool there, int k) {
-    const int64_t most = 0x7fff0000ll;  // the addresses of a tile end below (kMostLd)
-    const int64_t left = there ? all - at * step : 0;
-    const uint32_t records = left <= 0 ? 0u : (uint32_t)(left < most ? left : most);
-    source = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(first[low] + at * step), 0, (int)records, 0x00027000);
-    vnow = KC && at * kTileK + tail_chunk >= k ? 0x80000000u : voffset;
+  // The next step aimed at is step `at`, of `low`'s matrix.
+  __device__ __forceinline__ void begin(bool low, int at) {
+    base = first[low] + at * step;
+    records = KC ? full - at * (uint32_t)(kTileK * 2) : full;
+  }
+
+  // What the loads of the step read (the operand's last step?): nothing where `there` is false, zeros arrive.
+  __device__ __forceinline__ void aim(bool last, bool there) {
+    const uint32_t bytes = KC ? records : last ? tail : full;
+    // all lanes' are the same, and the loads want them in scalar registers: where the compiler has come to keep them in others it
+    // would loop over the lanes' values at every load
+    const uint64_t at = reinterpret_cast<uint64_t>(base);
+    const uint64_t low = (uint32_t)__builtin_amdgcn_readfirstlane((int)at), high = (uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32));
+    source = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(high << 32 | low), 0,
+                                               __builtin_amdgcn_readfirstlane((int)(there ? bytes : 0u)), 0x00027000);
+    vnow = KC && last ? vlast : voffset;
+    base += step;
+    records -= kTileK * 2;
   }
 
   // Load q of them into `lds` (this operand's part of a buffer).
@@ -279,7 +302,8 @@ struct OutEpilogue {
   MatList out, res;             // res: listed < 0 for none
   int64_t out_rs, out_cs, res_rs, res_cs;
   int out_type, res_type;
-  int lines;                    // rows of out and res are contiguous and begin at multiples of 16 bytes
+  int lines;                    // 1: rows of out and res are contiguous and begin at multiples of 16 bytes; 2: columns
+                                // do (and there is no mirror image); 0: neither
 
   template <int COLS>
   __device__ __forceinline__ void block(int z, int i0, int j0, float *sums, bool mirror, int lane) const {
@@ -289,18 +313,35 @@ struct OutEpilogue {
     if (lines && i0 + 32 <= rows && j0 + COLS <= cols) {
 #pragma unroll
       for (int turn = 0; turn < T::turns; ++turn) {
-        int i, j;
-        T::of_row(turn, lane, i, j);
-        float8v v = alpha * T::row_sums(sums, i, j);
-        i += i0;
-        j += j0;
+        int di, dj;
+        T::of_row(turn, lane, di, dj);
+        float8v v = alpha * T::row_sums(sums, di, dj);
+        const int i = i0 + di, j = j0 + dj;
         if (x) {
           const int64_t at = z * x_batch + (int64_t)i * x_ld + j;
           v += beta * (widen(*reinterpret_cast<const half8v *>(x + at)) + widen(*reinterpret_cast<const half8v *>(x_low + at)));
         }
         v *= gain;
+        if (lines == 2) {
+          T::put_row(sums, di, dj, v);
+          continue;
+        }
         if (r) v += keep * load_eight(r, i * res_rs + j, res_type);
         store_eight(o, i * out_rs + j, out_type, v);
+      }
+      if (lines == 2) {
+        lds_in_order();
+#pragma unroll
+        for (int turn = 0; turn < T::turns; ++turn) {
+          int i, j;
+          T::of_column(turn, lane, i, j);
+          float8v v = T::column_sums(sums, i, j);
+          i += i0;
+          j += j0;
+          if (r) v += keep * load_eight(r, j * res_cs + i, res_type);
+          store_eight(o, j * out_cs + i, out_type, v);
+        }
+        return;
       }
       if (!mirror) return;
 #pragma unroll 1
@@ -318,9 +359,10 @@ struct OutEpilogue {
     // one by one: the tile hangs over the matrix, or its rows are not lines
     const int turns = mirror ? 2 : 1;
     for (int turn = 0; turn < turns; ++turn) {
+      const bool down = (out_rs < out_cs) != (turn == 1);  // neighbouring lanes are neighbours of a column
 #pragma unroll 2
       for (int at = lane; at < 32 * COLS; at += 64) {
-        const int di = turn ? at & 31 : at / COLS, dj = turn ? at >> 5 : at % COLS;
+        const int di = down ? at & 31 : at / COLS, dj = down ? at >> 5 : at % COLS;
         const int i = i0 + di, j = j0 + dj;
         if (i >= rows || j >= cols) continue;
         float v = alpha * sums[di * T::row + dj];
@@ -393,14 +435,14 @@ constexpr int epilogue_cols() { return S::TN % 64 ? 32 : 64; }
 template <class S>
 constexpr int epilogue_halves() { return 2 * Stage<epilogue_cols<S>()>::floats; }
 
-// A wave's part of the tile, from row i0 and column j0 on.
-template <class S, class Epilogue>
-__device__ __forceinline__ void finish(const Epilogue &e, int z, int i0, int j0, const float16v (&acc)[S::FM][S::FN], bool mirror,
+// ROWS times 32 rows of a wave's part of the tile, from row i0 and column j0 on.
+template <class S, int ROWS, class Epilogue>
+__device__ __forceinline__ void finish(const Epilogue &e, int z, int i0, int j0, const float16v (&acc)[ROWS][S::FN], bool mirror,
                                        uint16_t *lds, int lane) {
   constexpr int kCols = epilogue_cols<S>();
   float *sums = reinterpret_cast<float *>(lds);
 #pragma unroll
-  for (int a = 0; a < S::FM; ++a)
+  for (int a = 0; a < ROWS; ++a)
 #pragma unroll
     for (int c = 0; c < S::TN; c += kCols) {
       // of a 32 x 32 block a lane holds row lane & 31: four times four neighbours, eight columns apart
@@ -438,14 +480,20 @@ __global__ __launch_bounds__(S::threads, S::W > 4 || S::stages * S::stage_halves
   lb.start(b, z, (int64_t)tj * S::BN, size.n, size.k, wave, lane);
   int at = begin % (steps ? steps : 1), part = begin / (steps ? steps : 1);  // what is loaded next: step of a part
   int left = all;
+  la.begin(part == 2, at);
+  lb.begin(part == 1, at);
 
-  auto aim = [&]() {  // no branches: the loads are to lie between the products
-    const bool there = left-- > 0;
-    la.aim(at, there && part == 2, there, size.k);
-    lb.aim(at, there && part == 1, there, size.k);
-    const bool wrap = at + 1 == steps;
-    at = wrap ? 0 : at + 1;
-    part += wrap;
+  auto aim = [&]() {
+    const bool there = left-- > 0, last = at + 1 == steps;
+    la.aim(last, there);
+    lb.aim(last, there);
+    ++at;
+    if (last) {
+      at = 0;
+      ++part;
+      la.begin(part == 2, 0);
+      lb.begin(part == 1, 0);
+    }
   };
   constexpr int kLoads = OpA::loads + OpB::loads;
   auto load = [&](uint16_t *buf, int l) {
@@ -459,57 +507,91 @@ __global__ __launch_bounds__(S::threads, S::W > 4 || S::stages * S::stage_halves
 #pragma unroll
     for (int j = 0; j < S::FN; ++j) acc[i][j] = float16v{};
 
-  // Fragments of 16 k are read while those before them are multiplied, also across the steps: a step's last quarter is
-  // multiplied while the first of the next one is read.  In front of that lies the step's one barrier: every wave has
-  // read all of the step's buffer and its own loads of the next one have arrived; behind it the buffer is loaded again, in
-  // this quarter and the next.  Reads and loads lie one by one between the products (a row of loads would hold the wave up for
-  // as long as the address unit takes over them), in the order written here.
-  short8v fa[2][S::FM], fb[2][S::FN];
-  constexpr int kProducts = S::FM * S::FN, kReads = S::FM + S::FN, kQuarters = kTileK / 16;
-  static_assert(kQuarters == 4 && kReads <= 2 * kProducts, "");
-  auto read = [&](const uint16_t *buf, int kk, int r) {
-    if (r < S::FN) fb[kk & 1][r] = OpB::read(buf + S::BM * kTileK, wn * S::TN + r * 32, kk, lane);
-    else fa[kk & 1][r - S::FN] = OpA::read(buf, wm * S::TM + (r - S::FN) * 32, kk, lane);
+  // Reads of LDS and loads into it lie one by one between the products, in the order written here (a row of loads would hold the
+  // wave up for as long as the address unit takes over them; the compiler would move reads to where they are used).
+  constexpr int kProducts = S::FM * S::FN, kReads = S::FM + S::FN, kQuarters = kTileK / 16, kAhead = (S::stages - 2) * kLoads;
+  constexpr int kSets = S::whole_steps ? 2 * kQuarters : 2;
+  short8v fa[kSets][S::FM], fb[kSets][S::FN];
+  auto read = [&](const uint16_t *buf, int kk, int set, int r) {
+    if (r < S::FN) fb[set][r] = OpB::read(buf + S::BM * kTileK, wn * S::TN + r * 32, kk, lane);
+    else fa[set][r - S::FN] = OpA::read(buf, wm * S::TM + (r - S::FN) * 32, kk, lane);
   };
-  // Quarter kk's products; between them the reads of quarter `then` and loads from..to - 1.
-  auto quarter = [&](int kk, const uint16_t *from, int then, uint16_t *into, int first, int last) {
+  // The products of `set`; between them the reads of quarter kk into set `to`, and loads first..last - 1.  The compiler lets a
+  // transposing read wait for all loads into LDS in front of it: with one of those the loads come behind the reads.
+  constexpr bool kPlain = AK && BK;
+  constexpr int kReadUp = kPlain ? kProducts : (kReads + 1) / 2;  // products that reads lie between
+  constexpr int kLoadFrom = kPlain ? 0 : kReadUp < kProducts ? kReadUp : kProducts - 1;
+  auto quarter = [&](int set, const uint16_t *from, int kk, int to, uint16_t *into, int first, int last) {
 #pragma unroll
     for (int p = 0; p < kProducts; ++p) {
 #pragma unroll
-      for (int r = p * 2; r < p * 2 + 2; ++r)
-        if (r < kReads) read(from, then, r);
+      for (int r = kReads * p / kReadUp; r < kReads * (p + 1) / kReadUp; ++r)
+        if (r < kReads) read(from, kk, to, r);
+      const int l0 = p < kLoadFrom ? 0 : (last - first) * (p - kLoadFrom) / (kProducts - kLoadFrom);
+      const int l1 = p < kLoadFrom ? 0 : (last - first) * (p - kLoadFrom + 1) / (kProducts - kLoadFrom);
 #pragma unroll
-      for (int l = 0; l < kLoads; ++l)
-        if (l >= first && l < last && (l - first) * kProducts / (last - first) == p) load(into, l);
+      for (int l = first + l0; l < first + l1; ++l) load(into, l);
       const int i = p / S::FN, j = p % S::FN;
-      acc[i][j] = mfma<BF>(fb[kk & 1][j], fa[kk & 1][i], acc[i][j]);
+      acc[i][j] = mfma<BF>(fb[set][j], fa[set][i], acc[i][j]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
+  // How many of a step's loads follow its barrier at once: with two buffers all, they are needed at the next one; with more the
+  // rest lie in the three quarters behind.
+  constexpr int kAtOnce = S::whole_steps || S::stages == 2 || !kPlain ? kLoads : kLoads / 4;
   if (all > 0) {
-    constexpr int kHalf = kLoads / 2, kAhead = (S::stages - 2) * kLoads;
 #pragma unroll
     for (int p = 0; p < S::stages; ++p) {
       aim();
 #pragma unroll
       for (int l = 0; l < kLoads; ++l)
-        if (p + 1 < S::stages || l < kHalf) load(s_buf + p * S::stage_halves, l);
+        if (p + 1 < S::stages || l < kAtOnce) load(s_buf + p * S::stage_halves, l);
     }
-    arrived<kAhead + kHalf>();
-#pragma unroll
-    for (int r = 0; r < kReads; ++r) read(s_buf, 0, r);
-    // step t's buffer, the next one's, and the one whose loads are half under way
-    int now = 0, next = S::stages > 1 ? S::stage_halves : 0, last = (S::stages - 1) * S::stage_halves;
-    for (int t = 0; t < all; ++t) {  // behind the last step zeros are loaded, and not multiplied
-      quarter(0, s_buf + now, 1, s_buf + last, kHalf, kLoads);
-      quarter(1, s_buf + now, 2, nullptr, 0, 0);
-      quarter(2, s_buf + now, 3, nullptr, 0, 0);
-      arrived<kAhead>();
-      aim();
-      quarter(3, s_buf + next, 0, s_buf + now, 0, kHalf);
-      last = now;
+    arrived<kAhead + kAtOnce>();
+    // step t's buffer, the next one's, and the one that is being loaded
+    int now = 0, next = S::stage_halves, into = (S::stages - 1) * S::stage_halves;
+    auto round = [&]() {
+      into = now;
       now = next;
       next = next + S::stage_halves == S::stages * S::stage_halves ? 0 : next + S::stage_halves;
+    };
+    if constexpr (S::whole_steps) {
+      // A step's products are too few to cover a quarter's reads: all of the next step is read while one is multiplied.  In front
+      // of that lies the step's one barrier: every wave has read this step whole, so its buffer is loaded again, and the next
+      // one has arrived.
+#pragma unroll
+      for (int kk = 0; kk < kQuarters; ++kk)
+#pragma unroll
+        for (int r = 0; r < kReads; ++r) read(s_buf, kk, kk, r);
+      for (int t = 0; t < all; t += 2) {  // an odd number: one step of zeros behind them
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          arrived<kAhead>();
+          aim();
+#pragma unroll
+          for (int kk = 0; kk < kQuarters; ++kk)
+            quarter(u * kQuarters + kk, s_buf + next, kk, (u ^ 1) * kQuarters + kk, s_buf + now,
+                    kPlain ? kLoads * kk / kQuarters : 0,
+                    kPlain ? kLoads * (kk + 1) / kQuarters : kk + 1 == kQuarters ? kLoads : 0);
+          round();
+        }
+      }
+    } else {
+      // Fragments of 16 k are read while those before them are multiplied, also across the steps: a step's last quarter is
+      // multiplied while the first of the next one is read.  In front of that lies the step's one barrier: every wave has
+      // read all of the step's buffer, so it is loaded again, and the next one has arrived.
+#pragma unroll
+      for (int r = 0; r < kReads; ++r) read(s_buf, 0, 0, r);
+      for (int t = 0; t < all; ++t) {  // behind the last step zeros are loaded, and not multiplied
+#pragma unroll
+        for (int kk = 0; kk + 1 < kQuarters; ++kk)
+          quarter(kk & 1, s_buf + now, kk + 1, ~kk & 1, s_buf + into, kAtOnce + (kLoads - kAtOnce) * kk / 3,
+                  kAtOnce + (kLoads - kAtOnce) * (kk + 1) / 3);
+        arrived<kAhead>();
+        aim();
+        quarter(1, s_buf + next, 0, 0, s_buf + now, 0, kAtOnce);
+        round();
+      }
     }
   }
 
@@ -528,36 +610,33 @@ __global__ __launch_bounds__(S::threads, S::W > 4 || S::stages * S::stage_halves
         }
     return;
   }
-  finish<S>(epilogue, z, ti * S::BM + wm * S::TM, tj * S::BN + wn * S::TN, acc, SYM && ti != tj, s_buf + wave * epilogue_halves<S>(), lane);
+  finish<S, S::FM>(epilogue, z, ti * S::BM + wm * S::TM, tj * S::BN + wn * S::TN, acc, SYM && ti != tj, s_buf + wave * epilogue_halves<S>(), lane);
 }
 
-// The sums of a tile's shares, in their order, and what becomes of them: a workgroup of one wave for each wave's part.
+// The sums of a tile's shares, in their order, and what becomes of them: a workgroup of one wave for every 32 rows of a wave's part.
 template <class S, bool SYM, class Epilogue>
 __global__ __launch_bounds__(64) void k_join(MatSize size, Epilogue epilogue) {
   __shared__ __attribute__((aligned(16))) uint16_t s_sums[epilogue_halves<S>()];
-  int z, ti, tj, wave;
-  tile_of<SYM>(size, S::W, wave, z, ti, tj);
-  const int lane = threadIdx.x;
+  int z, ti, tj, part;
+  tile_of<SYM>(size, S::W * S::FM, part, z, ti, tj);
+  const int wave = part / S::FM, rows = part % S::FM, lane = threadIdx.x;
   const float4v *from = reinterpret_cast<const float4v *>(size.partial + (int64_t)tile_number<SYM>(size, z, ti, tj) * size.splits * (S::BM * S::BN) +
-                                                          wave * S::wave_sums) + lane;
-  float16v acc[S::FM][S::FN];
+                                                          wave * S::wave_sums + rows * 32 * S::TN) + lane;
+  float16v acc[1][S::FN];
 #pragma unroll
-  for (int i = 0; i < S::FM; ++i)
-#pragma unroll
-    for (int j = 0; j < S::FN; ++j) acc[i][j] = float16v{};
+  for (int j = 0; j < S::FN; ++j) acc[0][j] = float16v{};
+#pragma unroll 4
   for (int share = 0; share < size.splits; ++share, from += S::BM * S::BN / 4) {
 #pragma unroll
-    for (int i = 0; i < S::FM; ++i)
+    for (int j = 0; j < S::FN; ++j)
 #pragma unroll
-      for (int j = 0; j < S::FN; ++j)
+      for (int q = 0; q < 4; ++q) {
+        const float4v f = from[(j * 4 + q) * 64];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float4v f = from[((i * S::FN + j) * 4 + q) * 64];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][j][q * 4 + e] += f[e];
-        }
+        for (int e = 0; e < 4; ++e) acc[0][j][q * 4 + e] += f[e];
+      }
   }
-  finish<S>(epilogue, z, ti * S::BM + wave / S::WN * S::TM, tj * S::BN + wave % S::WN * S::TN, acc, SYM && ti != tj, s_sums, lane);
+  finish<S, 1>(epilogue, z, ti * S::BM + wave / S::WN * S::TM + rows * 32, tj * S::BN + wave % S::WN * S::TN, acc, SYM && ti != tj, s_sums, lane);
 }
 
 template <class S, bool AK, bool BK, bool BF, bool SYM, class Epilogue>
@@ -566,11 +645,11 @@ inline int launch_tiles(MatSize size, const MatOperand &a, const MatOperand &b, 
   size.tiles_m = (size.m + S::BM - 1) / S::BM;
   size.tiles_n = (size.n + S::BN - 1) / S::BN;
   const int64_t tiles = (SYM ? (int64_t)size.tiles_m * (size.tiles_m + 1) / 2 : (int64_t)size.tiles_m * size.tiles_n) * size.batch;
-  if (tiles * (size.splits > S::W ? size.splits : S::W) > 0x7fffffffll) return fail(ZEN_EINVAL, "matrix product: too many tiles");
+  if (tiles * (size.splits > S::W * S::FM ? size.splits : S::W * S::FM) > 0x7fffffffll) return fail(ZEN_EINVAL, "matrix product: too many tiles");
   k_tiles<S, AK, BK, BF, SYM, Epilogue><<<dim3((unsigned)(tiles * size.splits)), dim3(S::threads), 0, stream>>>(size, a, b, e);
   ZEN_LAUNCH_CHECK("k_tiles");
   if (size.splits > 1) {
-    k_join<S, SYM, Epilogue><<<dim3((unsigned)(tiles * S::W)), dim3(64), 0, stream>>>(size, e);
+    k_join<S, SYM, Epilogue><<<dim3((unsigned)(tiles * S::W * S::FM)), dim3(64), 0, stream>>>(size, e);
     ZEN_LAUNCH_CHECK("k_join");
   }
   return ZEN_OK;
@@ -578,21 +657,22 @@ inline int launch_tiles(MatSize size, const MatOperand &a, const MatOperand &b, 
 
 // ---------------------------------------------------------------- which tiles
 
-// What a step of 64 k costs a compute unit, in us: measured with products of one to a few rounds of tiles (2048 x 2048 and 4096 x
-// 4096, k 1024 to 4096).  Large tiles read LDS and L2 least for their sums (4096^3: 126 us with 256, 190 us with 128, 309 us with 64);
-// small ones fill the card where there are few (1024 x 1024 x 4096: 85, 37 and 29 us).  A launch costs some us
-// apart from its steps, and so does joining the shares of tiles that are split.
+// What a step of 64 k costs a compute unit, in us: measured with products from one tile to some rounds of tiles (256 x 256 x 4096 to
+// 4096^3, k 1024 and 4096).  Large tiles read LDS and L2 least for their sums (4096^3: 124 us with 256, 130 with 128, 251
+// with 64); small ones fill the card where there are few (1024 x 1024 x 4096: 79, 32 and 20 us).  With a tile on every unit the
+// L2s bound the small ones (12 to 16 TB/s).  A launch costs some us apart from its steps, and so does joining the shares of
+// tiles that are split.
 struct TileCost {
   int side;
-  int at_once;       // workgroups that a compute unit holds
-  float step, lone;  // us, with that many on every compute unit, or one at most
-  float launch;      // us, with the epilogue
-  bool k_only;       // operands with k contiguous only
+  int at_once;           // workgroups that a compute unit holds
+  float lone, one, all;  // us a step: a workgroup by itself; one on every unit; at_once on every unit
+  float launch;          // us, with the epilogue
+  bool k_only;           // operands with k contiguous only
 };
 constexpr TileCost kTileCosts[] = {
-    {256, 1, 1.85f, 1.50f, 10.f, false}, {192, 1, 1.20f, 1.00f, 8.f, true},
-    {128, 2, 1.10f, 1.10f, 6.f, false}, {128, 1, 0.66f, 0.45f, 6.f, false}, {64, 2, 0.60f, 0.34f, 4.f, false}};
-constexpr int kMostSplits = 16;
+    {256, 1, 1.10f, 1.85f, 1.85f, 9.f, false}, {192, 1, 0.75f, 1.20f, 1.20f, 7.f, true},
+    {128, 2, 0.95f, 0.95f, 1.05f, 6.f, false}, {128, 1, 0.37f, 0.64f, 0.64f, 5.f, false}, {64, 2, 0.17f, 0.25f, 0.48f, 4.f, false}};
+constexpr int kMostSplits = 24;
 
 struct TilePlan {
   int side, at_once, splits;
@@ -609,10 +689,11 @@ inline TilePlan plan_tiles(int64_t m, int64_t n, int64_t k, int parts, int64_t b
     const int64_t tiles = (sym ? down * (down + 1) / 2 : down * across) * batch;
     for (int splits = 1; splits <= kMostSplits && (splits == 1 || (tiles * splits <= 512 && steps / splits >= 4)); ++splits) {
       const int64_t groups = tiles * splits;
-      const double step = groups <= 256 ? c.lone + (c.step / c.at_once - c.lone) * (c.at_once == 1 ? groups / 256.0 : 0.0) : c.step;
-      const double rounds = groups <= 256 ? 1.0 : (double)ceil_div(groups, 256 * c.at_once);
+      // whole rounds, and a last one of so many a unit
+      const int64_t slots = 256 * c.at_once, whole = groups <= 256 ? 0 : groups / slots, rest = groups - whole * slots;
+      const double last = rest == 0 ? 0.0 : rest <= 256 ? c.lone + (c.one - c.lone) * rest / 256.0 : c.all;
       const double bytes = splits > 1 ? 4.0 * groups * c.side * c.side : 0.0;
-      const double us = rounds * (double)ceil_div(steps, splits) * step + c.launch + (splits > 1 ? 5.0 + bytes / 2e6 : 0.0);
+      const double us = (whole * c.all + last) * (double)ceil_div(steps, splits) + c.launch + (splits > 1 ? 4.0 + bytes / 2e6 : 0.0);
       if (us < least) {
         least = us;
         best = {c.side, c.at_once, splits, (size_t)bytes};
