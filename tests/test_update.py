@@ -494,11 +494,11 @@ def update_like(m, n, seed, kind="gauss"):
 def room_of(u, dtype, **more):
     """Tolerance of a result of `dtype`, 2-norm, relative: rounding the result, and twice what the operands' roundings do (their
     effect depends on where they fall; a second run of the same ones with other inputs differs by some ten per cent).
-    fp32: four times what fp32 products do (an operand of 22 bits instead of 24 is off four times as far)."""
+    fp32 and fp16: four times what fp32 products do (an operand of 22 bits instead of 24 is off four times as far)."""
     exact = newton_schulz(u, **more)
-    if dtype == F32:
+    if dtype != BF16 and not more:
         fp32 = newton_schulz_fp32(u if u.shape[0] <= u.shape[1] else u.T)
-        return exact, U[F32] + 4 * max(off(fp32 if u.shape[0] <= u.shape[1] else fp32.T, exact), 4 * U[F32])
+        return exact, U[dtype] + 4 * max(off(fp32 if u.shape[0] <= u.shape[1] else fp32.T, exact), 4 * U[F32])
     return exact, U[dtype] + 2 * off(newton_schulz(u, half=True, **more), exact)
 
 

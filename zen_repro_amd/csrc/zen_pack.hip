@@ -8,9 +8,19 @@ namespace {
 
 constexpr int kSide = 64;
 
-__global__ __launch_bounds__(256) void k_pack(PackArgs p) {
+struct Two {
+  PackArgs of[2];
+  int64_t blocks[2], across[2], down[2];
+};
+
+__global__ __launch_bounds__(256) void k_pack(Two two) {
   __shared__ uint16_t s_tile[kSide][kSide + 2];  // a row is 33 words: columns lie in different banks
-  const int z = blockIdx.z, i0 = blockIdx.y * kSide, j0 = blockIdx.x * kSide, tid = threadIdx.x;
+  const int which = (int64_t)blockIdx.x >= two.blocks[0];
+  const PackArgs &p = two.of[which];
+  int64_t at_block = (int64_t)blockIdx.x - (which ? two.blocks[0] : 0);
+  const int tid = threadIdx.x, j0 = (int)(at_block % two.across[which]) * kSide;
+  at_block /= two.across[which];
+  const int i0 = (int)(at_block % two.down[which]) * kSide, z = (int)(at_block / two.down[which]);
   const uint16_t *in = reinterpret_cast<const uint16_t *>(p.in.of(z));
   const bool across = p.cs <= p.rs;  // neighbours in memory are neighbours of a row
 #pragma unroll
@@ -31,10 +41,17 @@ __global__ __launch_bounds__(256) void k_pack(PackArgs p) {
 
 }  // namespace
 
-int pack_matrices(const PackArgs &p, hipStream_t stream) {
-  const int64_t across = ceil_div(p.ld, kSide), down = ceil_div(p.rows, kSide);
-  if (across > 0x7fffffffll || down > 65535 || p.batch > 65535) return fail(ZEN_EINVAL, "matrix product: too many rows");
-  k_pack<<<dim3((unsigned)across, (unsigned)down, (unsigned)p.batch), dim3(256), 0, stream>>>(p);
+int pack_matrices(const PackArgs *args, int count, hipStream_t stream) {
+  Two two = {};
+  for (int i = 0; i < count; ++i) {
+    two.of[i] = args[i];
+    two.across[i] = ceil_div(args[i].ld, kSide);
+    two.down[i] = ceil_div(args[i].rows, kSide);
+    if (two.down[i] > 0x7fffffffll / two.across[i]) return fail(ZEN_EINVAL, "matrix product: too many rows");
+    two.blocks[i] = two.across[i] * two.down[i] * args[i].batch;
+  }
+  if (two.blocks[0] + two.blocks[1] > 0x7fffffffll) return fail(ZEN_EINVAL, "matrix product: too many rows");
+  k_pack<<<dim3((unsigned)(two.blocks[0] + two.blocks[1])), dim3(256), 0, stream>>>(two);
   ZEN_LAUNCH_CHECK("k_pack");
   return ZEN_OK;
 }

@@ -35,10 +35,10 @@ size_t room(const Side &s, int64_t batches) {
   return s.packed ? align_up((size_t)s.rows * s.ld * batches * 2, 256) : 0;
 }
 
-int lay_out(Side &s, int64_t batches, Carver &cv, hipStream_t stream) {
-  if (!s.packed) return ZEN_OK;
-  uint16_t *to = cv.take<uint16_t>((size_t)s.rows * s.ld * batches);
-  PackArgs p = {};
+// How the operand is laid out, if it is; the side is then read from there.
+bool lay_out(Side &s, int64_t batches, Carver &cv, PackArgs &p) {
+  if (!s.packed) return false;
+  p = {};
   p.in.base = static_cast<char *>(const_cast<void *>(s.p));
   p.in.stride = s.batch * 2;
   p.rs = s.row;
@@ -46,12 +46,12 @@ int lay_out(Side &s, int64_t batches, Carver &cv, hipStream_t stream) {
   p.rows = (int)s.rows;
   p.cols = (int)s.k;
   p.batch = (int)batches;
-  p.out = to;
+  p.out = cv.take<uint16_t>((size_t)s.rows * s.ld * batches);
   p.ld = s.ld;
   p.out_batch = s.rows * s.ld;
-  s.p = to;
+  s.p = p.out;
   s.batch = p.out_batch;
-  return pack_matrices(p, stream);
+  return true;
 }
 
 bool known(int type) { return type == ZEN_F32 || type == ZEN_BF16 || type == ZEN_F16; }
@@ -115,8 +115,11 @@ int zen_product(const zen_product_args *p) {
   const TilePlan how = plan(*p, sa, sb);
   Carver cv(p->workspace);
   if (p->k > 0) {
-    if (const int rc = lay_out(sa, p->batch, cv, s)) return rc;
-    if (const int rc = lay_out(sb, p->batch, cv, s)) return rc;
+    PackArgs pack[2];
+    int packs = lay_out(sa, p->batch, cv, pack[0]) ? 1 : 0;
+    packs += lay_out(sb, p->batch, cv, pack[packs]) ? 1 : 0;
+    if (packs)
+      if (const int rc = pack_matrices(pack, packs, s)) return rc;
   }
   const MatSize size = {(int)p->m, (int)p->n, (int)p->k, 0, 0, (int)p->batch, 1, 1, nullptr};
   float *partial = reinterpret_cast<float *>(cv.base + cv.used);

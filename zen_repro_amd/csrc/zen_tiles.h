@@ -305,9 +305,10 @@ struct OutEpilogue {
   int lines;                    // 1: rows of out and res are contiguous and begin at multiples of 16 bytes; 2: columns
                                 // do (and there is no mirror image); 0: neither
 
-  template <int COLS>
+  template <int COLS, int AT>
   __device__ __forceinline__ void block(int z, int i0, int j0, float *sums, bool mirror, int lane) const {
     using T = Stage<COLS>;
+    if (i0 >= rows || j0 >= cols) return;
     char *o = out.of(z);
     const char *r = res.listed >= 0 ? res.of(z) : nullptr;
     if (lines && i0 + 32 <= rows && j0 + COLS <= cols) {
@@ -360,20 +361,29 @@ struct OutEpilogue {
     const int turns = mirror ? 2 : 1;
     for (int turn = 0; turn < turns; ++turn) {
       const bool down = (out_rs < out_cs) != (turn == 1);  // neighbouring lanes are neighbours of a column
-#pragma unroll 2
-      for (int at = lane; at < 32 * COLS; at += 64) {
-        const int di = down ? at & 31 : at / COLS, dj = down ? at >> 5 : at % COLS;
-        const int i = i0 + di, j = j0 + dj;
-        if (i >= rows || j >= cols) continue;
-        float v = alpha * sums[di * T::row + dj];
-        if (x) {
-          const int64_t from = z * x_batch + (int64_t)i * x_ld + j;
-          v += beta * ((float)x[from] + (float)x_low[from]);
+      for (int base = lane; base < 32 * COLS; base += 64 * AT) {
+        float v[AT];
+        int64_t to[AT];
+        bool there[AT];
+#pragma unroll
+        for (int u = 0; u < AT; ++u) {  // no branches: what lies beyond the matrix reads its last row or column
+          const int at = base + u * 64;
+          const int di = down ? at & 31 : at / COLS, dj = down ? at >> 5 : at % COLS;
+          there[u] = i0 + di < rows && j0 + dj < cols;
+          const int i = i0 + di < rows ? i0 + di : rows - 1, j = j0 + dj < cols ? j0 + dj : cols - 1;
+          const int64_t to_i = turn ? j : i, to_j = turn ? i : j;
+          v[u] = alpha * sums[di * T::row + dj];
+          if (x) {
+            const int64_t from = z * x_batch + (int64_t)i * x_ld + j;
+            v[u] += beta * ((float)x[from] + (float)x_low[from]);
+          }
+          v[u] *= gain;
+          if (r) v[u] += keep * load_value(r, to_i * res_rs + to_j * res_cs, res_type);
+          to[u] = to_i * out_rs + to_j * out_cs;
         }
-        v *= gain;
-        const int64_t to_i = turn ? j : i, to_j = turn ? i : j;
-        if (r) v += keep * load_value(r, to_i * res_rs + to_j * res_cs, res_type);
-        store_value(o, to_i * out_rs + to_j * out_cs, out_type, v);
+#pragma unroll
+        for (int u = 0; u < AT; ++u)
+          if (there[u]) store_value(o, to[u], out_type, v[u]);
       }
     }
   }
@@ -395,7 +405,7 @@ struct KeepEpilogue {
     if (low) *reinterpret_cast<half8v *>(low + at) = __builtin_convertvector(v - widen(h), half8v);
   }
 
-  template <int COLS>
+  template <int COLS, int AT>
   __device__ __forceinline__ void block(int z, int i0, int j0, float *sums, bool mirror, int lane) const {
     using T = Stage<COLS>;
     if (i0 >= rows || j0 >= cols) return;
@@ -440,6 +450,8 @@ template <class S, int ROWS, class Epilogue>
 __device__ __forceinline__ void finish(const Epilogue &e, int z, int i0, int j0, const float16v (&acc)[ROWS][S::FN], bool mirror,
                                        uint16_t *lds, int lane) {
   constexpr int kCols = epilogue_cols<S>();
+  // elements on their way together where they go one by one: many where the code is laid out few times
+  constexpr int kAtOnce = ROWS * S::TN / kCols <= 2 ? 8 : 2;
   float *sums = reinterpret_cast<float *>(lds);
 #pragma unroll
   for (int a = 0; a < ROWS; ++a)
@@ -455,7 +467,7 @@ __device__ __forceinline__ void finish(const Epilogue &e, int z, int i0, int j0,
               float4v{f[q * 4], f[q * 4 + 1], f[q * 4 + 2], f[q * 4 + 3]};
         }
       lds_in_order();
-      e.template block<kCols>(z, i0 + a * 32, j0 + c, sums, mirror, lane);
+      e.template block<kCols, kAtOnce>(z, i0 + a * 32, j0 + c, sums, mirror, lane);
       lds_in_order();
     }
 }
@@ -733,6 +745,6 @@ struct PackArgs {
   uint16_t *out;
   int64_t ld, out_batch;
 };
-int pack_matrices(const PackArgs &args, hipStream_t stream);
+int pack_matrices(const PackArgs *args, int count, hipStream_t stream);  // one or two of them, one launch
 
 }  // namespace zen

@@ -18,8 +18,8 @@ class Muon(torch.optim.Optimizer):
     momentum, nesterov, weight_decay, steps, coefficients, eps   see momentum_update and orthogonal_step
     match_rms     a number r: scale = r * sqrt(max(rows, cols)), which gives every update's elements an RMS of about
                   r * lr whatever the matrix' shape; None: scale = sqrt(max(1, rows / cols))
-    precision     of the orthogonalisation, and the type in which the momentum hands the update on (default bfloat16;
-                  float32 for fp32's accuracy throughout)
+    precision     of the orthogonalisation (see orthogonal_step), and the type in which the momentum hands the update
+                  on (default bfloat16; float32 for fp32's accuracy throughout)
     The momentum is kept in fp32.  Parameters of one shape go through the orthogonalisation together."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,

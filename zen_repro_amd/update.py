@@ -126,7 +126,7 @@ def _orthogonal(what, updates, outs, steps, coefficients, eps, precision, weight
     device = updates[0].device
     rc = _called(updates[0], _lib.host.orthogonal, L.zen_orthogonal, L.zen_orthogonal_workspace,
                  lambda nbytes: _workspace(device, "orthogonal", nbytes), what, updates, outs, int(steps), *coefficients,
-                 eps, precision == torch.float32, weights, keep, gain)
+                 eps, precision != torch.bfloat16, weights, keep, gain)
     if rc:
         _lib.check(rc, what)
 
@@ -137,8 +137,8 @@ def orthogonalize(update, steps=5, coefficients=COEFFICIENTS, eps=1e-7, dtype=No
 
     update  a matrix, a stack (3-D) or a list of matrices of one shape; fp32, bf16 or fp16, any strides.  Many small matrices
             are quicker in one call than one by one
-    dtype   the result's type (default: the update's).  It decides the precision: for fp32 every product's operands
-            have 22 bits (three products of fp16), else fp16 operands and an iterate of 22 bits
+    dtype   the result's type (default: the update's).  It decides the precision: for bf16 the products' operands are
+            fp16, for fp32 and fp16 they have 22 bits (three products of fp16 each); the iterate has 22 bits
     out     where the result goes, of the update's shape (a list for a list); may be the update itself"""
     updates = _matrices(update, "update")
     listed = isinstance(update, (list, tuple))
@@ -163,7 +163,7 @@ def orthogonal_step(weight, update, lr, weight_decay=0.0, scale=1.0, steps=5, co
 
     weight, update  a matrix each, a stack or a list of matrices of one shape
     precision       fp32, bf16 or fp16: how precise the orthogonalised update is (see orthogonalize).  Default: as the
-                    weight's type asks for; bf16 for fp32 weights is some two to three times quicker"""
+                    weight's type asks for; bf16 for fp32 weights is up to two and a half times quicker"""
     weights, updates = _matrices(weight, "weight"), _matrices(update, "update")
     if len(weights) != len(updates):
         raise ValueError(f"orthogonal_step: {len(weights)} weights and {len(updates)} updates")
