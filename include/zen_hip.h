@@ -718,7 +718,7 @@ int zen_momentum_lists(void *momentum, int momentum_dtype, const void *const *id
  * where one of the two is 1 and addresses and the other stride are multiples of 16 bytes (for b with b_rs == 1, and a with
  * a_cs == 1, k too), they are read as they lie, else they are laid out in the workspace first.  c (null: none) and out: any
  * strides, ZEN_F32, ZEN_BF16 or ZEN_F16; out may be c itself (the same addresses and strides), else it overlaps nothing.
- * symmetric: the caller vouches that a b is (m == n): half of it is computed and mirrored.
+ * symmetric: the caller vouches that a b is (m == n): half of it is computed and mirrored.  k is at most 2^21.
  */
 typedef struct zen_product_args {
   const void *a;

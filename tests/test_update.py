@@ -70,7 +70,7 @@ def product_args(**more):
 
 
 def test_product_refusals_of_the_library(L):
-    for bad in (dict(m=-1), dict(k=1 << 31), dict(dtype=0), dict(out_dtype=3), dict(c=256, c_dtype=9), dict(symmetric=1, n=32),
+    for bad in (dict(m=-1), dict(k=1 << 31), dict(k=(1 << 21) + 8, a_rs=1 << 22), dict(dtype=0), dict(out_dtype=3), dict(c=256, c_dtype=9), dict(symmetric=1, n=32),
                 dict(a_rs=-64), dict(out=None), dict(b=None), dict(batch=1 << 20)):
         assert L.zen_product(product_args(**bad)) == _lib.EINVAL, bad
     assert L.zen_product(None) == _lib.EINVAL
@@ -117,6 +117,16 @@ def test_muon_takes_matrices():
         zen.Muon([torch.nn.Parameter(torch.zeros(4, 4))], lr=-1)
     with pytest.raises(TypeError):
         zen.Muon([torch.nn.Parameter(torch.zeros(4, 4))], precision=torch.float64)
+
+
+def test_muon_keeps_its_momentum_in_fp32():
+    params = [torch.nn.Parameter(torch.zeros(4, 4, dtype=BF16)) for _ in range(2)]
+    opt = zen.Muon(params)
+    opt.state[params[1]]["momentum"] = torch.full((4, 4), 1.0 + 2.0 ** -20)
+    other = zen.Muon([torch.nn.Parameter(torch.zeros(4, 4, dtype=BF16)) for _ in range(2)])
+    other.load_state_dict(opt.state_dict())
+    got = other.state[other.param_groups[0]["params"][1]]["momentum"]
+    assert got.dtype == F32 and torch.equal(got, opt.state[params[1]]["momentum"])
 
 
 # -------------------------------------------------------------------- momentum
@@ -619,6 +629,24 @@ def test_orthogonal_refusals():
 
 
 # --------------------------------------------------------------------- together
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    """Calls in flight on two streams at a time, from one thread, keep apart."""
+    us = [update_like(700, 900, 155 + i).to(BF16) for i in range(2)]
+    a, b = normal((400, 1001), 157, F16)[:, 1:], normal((1000, 300), 158, F16)
+    want = [zen.orthogonalize(u) for u in us], zen.product(a, b)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for s, u in zip(streams, us):
+            with torch.cuda.stream(s):
+                got.append((zen.orthogonalize(u), zen.product(a, b)))
+    torch.cuda.synchronize()
+    for i, (o, p) in enumerate(got):
+        assert torch.equal(o, want[0][i % 2]) and torch.equal(p, want[1])
 
 
 @pytest.mark.gpu

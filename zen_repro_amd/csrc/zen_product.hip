@@ -107,6 +107,7 @@ int zen_product(const zen_product_args *p) {
   if (const int rc = check(p)) return rc;
   if (p->m == 0 || p->n == 0 || p->batch == 0) return ZEN_OK;
   if (!p->out || (p->k > 0 && (!p->a || !p->b))) return fail(ZEN_EINVAL, "zen_product: null pointer");
+  if (p->k > kMostLd) return fail(ZEN_EINVAL, "zen_product: k is at most 2^21");
   const size_t need = zen_product_workspace(p);
   if (need && !p->workspace) return fail(ZEN_EINVAL, "zen_product: null pointer");
   if (p->workspace_bytes < need) return fail(ZEN_EWORKSPACE, "zen_product: workspace too small");

@@ -37,6 +37,16 @@ class Muon(torch.optim.Optimizer):
             self.param_groups.pop()
             raise ValueError("Muon: parameters have two dimensions; give the others to another optimiser")
 
+    def load_state_dict(self, state_dict):
+        """torch's gives every state its parameter's type; the momentum stays fp32."""
+        super().load_state_dict(state_dict)
+        saved = [i for group in state_dict["param_groups"] for i in group["params"]]
+        own = [p for group in self.param_groups for p in group["params"]]
+        for i, p in zip(saved, own):
+            momentum = state_dict["state"].get(i, {}).get("momentum")
+            if momentum is not None:
+                self.state[p]["momentum"] = momentum.to(device=p.device, dtype=torch.float32, copy=True)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None

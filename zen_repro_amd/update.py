@@ -3,21 +3,17 @@ merged lists themselves), matrix products with a residual, and the orthogonalisa
 steps.  `Muon` (muon.py) is the optimiser made of them.
 
 Every call works on the current stream of its tensors' device, waits for nothing and can be captured into a graph
-(a captured call has a workspace of its own).  None of them is differentiated: with gradients enabled, tensors that require
+(where a status is returned, after _lib.zeros.fresh(device) at the start of the capture).  None of them is differentiated: with gradients enabled, tensors that require
 them are refused."""
 import torch
 
 from . import _lib
 
 
-def _workspace(device, name, nbytes):
-    """The calling thread's buffer of that name.  A captured call's belongs to its graph: two graphs may replay side by
-    side, and the thread's buffer may be replaced by a larger one."""
-    if not nbytes:
-        return None
-    if torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return _lib.scratch.get(device, name, nbytes)
+def _workspace(device, nbytes):
+    """From torch's allocator, in the order of the current stream: calls on several streams, or captured into several
+    graphs, never share one."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 def _called(t, call, *args):
@@ -69,7 +65,7 @@ def momentum_update_sparse(momentum, indices_tensors, values_tensors, mu=0.95, n
     L = _lib.lib()
     ws = None
     if momentum.is_cuda:
-        ws = _workspace(momentum.device, "momentum", L.zen_momentum_lists_workspace(momentum.numel(), len(indices)))
+        ws = _workspace(momentum.device, L.zen_momentum_lists_workspace(momentum.numel(), len(indices)))
     rc, out, status = _called(momentum, _lib.host.momentum_lists, L.zen_momentum_lists, _lib.zeros.native(), momentum, indices,
                               values, mu, nesterov, counted, counts, dtype, out, ws)
     if rc:
@@ -85,7 +81,7 @@ def product(a, b, residual=None, alpha=1.0, beta=1.0, symmetric=False, dtype=Non
 
     a, b       bf16 or fp16 matrices (m x k and k x n), or stacks of as many; any strides.  Where rows or columns are contiguous
                and begin at multiples of 16 bytes they are read as they lie (a transposed view costs nothing), else
-               laid out first
+               laid out first.  k is at most 2^21
     residual   m x n (or a stack), fp32, bf16 or fp16, any strides
     symmetric  the caller vouches that a @ b is symmetric (a matrix and its own transpose, powers of a symmetric
                matrix): half of it is computed and mirrored
@@ -93,7 +89,7 @@ def product(a, b, residual=None, alpha=1.0, beta=1.0, symmetric=False, dtype=Non
     out        where the result goes, any strides; may be the residual itself"""
     L = _lib.lib()
     rc, out = _called(a, _lib.host.product, L.zen_product, L.zen_product_workspace,
-                      lambda nbytes: _workspace(a.device, "product", nbytes), a, b, residual, alpha, beta, symmetric, dtype, out)
+                      lambda nbytes: _workspace(a.device, nbytes), a, b, residual, alpha, beta, symmetric, dtype, out)
     if rc:
         _lib.check(rc, "product")
     return out
@@ -125,7 +121,7 @@ def _orthogonal(what, updates, outs, steps, coefficients, eps, precision, weight
     L = _lib.lib()
     device = updates[0].device
     rc = _called(updates[0], _lib.host.orthogonal, L.zen_orthogonal, L.zen_orthogonal_workspace,
-                 lambda nbytes: _workspace(device, "orthogonal", nbytes), what, updates, outs, int(steps), *coefficients,
+                 lambda nbytes: _workspace(device, nbytes), what, updates, outs, int(steps), *coefficients,
                  eps, precision != torch.bfloat16, weights, keep, gain)
     if rc:
         _lib.check(rc, what)
