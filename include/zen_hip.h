@@ -9,7 +9,8 @@
  *
  * Conventions
  *   - every pointer is DEVICE memory unless a comment says "host";
- *   - `dtype` is ZEN_F32 or ZEN_BF16 (bf16 as 16-bit patterns);
+ *   - `dtype` is ZEN_F32 or ZEN_BF16 (bf16 as 16-bit patterns), or ZEN_F16 where a
+ *     comment says so;
  *   - `stream` is a hipStream_t (NULL = the null stream);
  *   - the return value is a host-side code (ZEN_OK, ZEN_E...); conditions only
  *     the device can see are OR-ed into `*status` (device int32, written by
@@ -58,8 +59,9 @@ extern "C" {
  *    element (zen_bitmap_dense_dict_bytes): built anew, not kept from an older
  *    library
  * 11: such a dictionary's chunk words have 32 bits: built anew
+ * 12: ZEN_F16, zen_momentum, zen_momentum_lists, zen_product, zen_orthogonal
  */
-#define ZEN_ABI_VERSION 11
+#define ZEN_ABI_VERSION 12
 
 #define ZEN_F32 0
 #define ZEN_BF16 1

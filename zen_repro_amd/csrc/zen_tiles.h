@@ -11,7 +11,7 @@
 // What bounds it: with 256 x 256 tiles a step's products take a compute unit 2048 cycles, of some 2900 (8192^3, k contiguous:
 // matrix cores busy 71 % of the cycles, LDS 20 %, and a clock that the power limit holds at 1.5 to 1.9 GHz: 1110 to 1260
 // TFLOP/s; without the loads, 1550).  What mattered most: reads, loads and products in an order of our own, one by one (the
-// compiler's: 1.83 against 1.50 million cycles at that size), and reads of LDS without bank conflicts.
+// compiler's: 1.79 against 1.50 million cycles at that size), and reads of LDS without bank conflicts.
 //
 // LDS layout: a row of 64 k is eight 16-byte pieces; piece c of row r lies in place c ^ key(r).  With k as the stride a row
 // holds the tile's i or j, and piece c of row k lies in place(k, c).  Both spread what lanes read at the same time (32 rows at one c;
