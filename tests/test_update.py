@@ -382,6 +382,32 @@ def test_product_strides_types_and_the_residual_in_place(out, res):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_product_turned_results_and_residuals_that_are_one_row(dtype):
+    m, n, k = 200, 328, 136
+    a, b = normal((m, k), 63, BF16), normal((k, n), 64, BF16)
+    c = normal((n, m), 65, dtype).t()
+    for residual in (None, c, normal((1, n), 66, dtype).expand(m, n), normal((m, 1), 67, dtype).expand(m, n)):
+        for out in (torch.empty(n, m, device="cuda", dtype=dtype).t(), torch.empty(m, n, device="cuda", dtype=dtype)):
+            zen.product(a, b, residual=residual, beta=2.0, out=out)
+            product_check(out, a, b, residual, 1.0, 2.0)
+    own = c.clone()
+    assert own.stride() == c.stride()
+    zen.product(a, b, residual=own, out=own)
+    product_check(own, a, b, c, 1.0, 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [64, 200, 203])
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_product_symmetric_into_its_residual(m, dtype):
+    a, c = normal((m, 72), 68, F16), normal((m, m), 69, dtype)
+    own = c.clone()
+    zen.product(a, a.t(), residual=own, alpha=0.5, beta=-1.0, symmetric=True, out=own)
+    product_check(own, a, a.t(), c, 0.5, -1.0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("turned", [False, True])
 @pytest.mark.parametrize("stack,m,n,k", [(1, 64, 64, 64), (3, 100, 72, 200), (5, 129, 257, 64), (7, 8, 8, 8)])
 def test_product_of_stacks(stack, m, n, k, turned):
@@ -512,7 +538,7 @@ def room_of(u, dtype, **more):
     return exact, U[dtype] + 2 * off(newton_schulz(u, half=True, **more), exact)
 
 
-SHAPES = [(1, 1), (1, 40), (1100, 1030), (700, 2100), (3, 2), (64, 64), (65, 63), (128, 128), (48, 500), (500, 48), (200, 333), (300, 257), (130, 1030)]
+SHAPES = [(1, 1), (1, 40), (320, 128), (1024, 256), (40, 1), (1100, 1030), (700, 2100), (3, 2), (64, 64), (65, 63), (128, 128), (48, 500), (500, 48), (200, 333), (300, 257), (130, 1030)]
 
 
 @pytest.mark.gpu

@@ -11,8 +11,8 @@
 // amplifies rounding (errors against 64 bits, Gaussian update 1024 x 1024: bf16 2e-2, fp16 1e-3).  Where a direction starts
 // small it grows by `a` a step, and so does the noise that rounding X adds to it; so X is carried on as two fp16 (22 bits) and
 // only the products see 11 of them.  The last two steps are written as X + (b A + c A A + (a - 1) I) X: there
-// the singular values are near 1, the bracket is near zero, and so is what rounding it does.  With `precise` the
-// products see 22 bits of every operand too: A B + A B' + A' B, what is left out is below 2^-22.
+// the singular values are near 1, the bracket is near zero, and so is what rounding it does.  With `precise`
+// (results of fp32 and fp16) the products see 22 bits of every operand too: A B + A B' + A' B, what is left out is below 2^-22.
 #include "zen_tiles.h"
 
 namespace zen {
@@ -21,7 +21,6 @@ namespace {
 constexpr float kUnit = 1024.f;
 constexpr int kSquareBlock = 256;
 constexpr int kMostShares = 1024;  // workgroups to a matrix' sum of squares
-
 
 // Sums of squares in fp64 (an fp32 square overflows from 2^64 on), one a workgroup, in a fixed order.  `slow` lines of `fast`
 // values; wide: a line is contiguous and begins at a multiple of 16 bytes.  Bound by the read.
@@ -231,7 +230,8 @@ int chunk(const zen_orthogonal_args &p, const Room &r, int64_t first, int batch,
   const int parts = p.precise ? 3 : 1;
   const int m = (int)r.m, n = (int)r.n;
   const int64_t mm = r.m * r.m, mn = r.m * r.n;
-  const MatSize gram = {m, m, n, 0, 0, batch, parts, 1, nullptr}, square = {m, m, m, 0, 0, batch, parts, 1, nullptr}, apply = {m, n, m, 0, 0, batch, parts, 1, nullptr};
+  const MatSize gram = {m, m, n, 0, 0, batch, parts, 1, nullptr}, square = {m, m, m, 0, 0, batch, parts, 1, nullptr},
+                apply = {m, n, m, 0, 0, batch, parts, 1, nullptr};
   for (int step = 0; step < p.steps; ++step) {
     const int at = step & 1;
     const bool near = step >= p.steps - 2;
