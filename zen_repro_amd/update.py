@@ -3,8 +3,8 @@ merged lists themselves), matrix products with a residual, and the orthogonalisa
 steps.  `Muon` (muon.py) is the optimiser made of them.
 
 Every call works on the current stream of its tensors' device, waits for nothing and can be captured into a graph
-(where a status is returned, after _lib.zeros.fresh(device) at the start of the capture).  None of them is differentiated: with gradients enabled, tensors that require
-them are refused."""
+(where a status is returned, after _lib.zeros.fresh(device) at the start of the capture).  None of them is
+differentiated: with gradients enabled, tensors that require them are refused."""
 import torch
 
 from . import _lib
@@ -82,7 +82,7 @@ def product(a, b, residual=None, alpha=1.0, beta=1.0, symmetric=False, dtype=Non
     a, b       bf16 or fp16 matrices (m x k and k x n), or stacks of as many; any strides.  Where rows or columns are contiguous
                and begin at multiples of 16 bytes they are read as they lie (a transposed view costs nothing), else
                laid out first.  k is at most 2^21
-    residual   m x n (or a stack), fp32, bf16 or fp16, any strides
+    residual   m x n (or a stack), fp32, bf16 or fp16, any strides.  It is read whatever beta is: NaN in it stays NaN
     symmetric  the caller vouches that a @ b is symmetric (a matrix and its own transpose, powers of a symmetric
                matrix): half of it is computed and mirrored
     dtype      the result's type (default: the residual's, else a's): fp32, bf16 or fp16
