@@ -36,18 +36,11 @@ __global__ __launch_bounds__(kSquareBlock) void k_squares(MatList in, int64_t sl
   for (int64_t at = first + threadIdx.x; at < last; at += kSquareBlock) {
     const int64_t i = at / pieces;
     const int j = (int)(at - i * pieces) * 8;
-    if (wide && j + 8 <= fast) {
-      const float8v v = load_eight(p, i * slow_stride + j, dtype);
+    const float8v v = wide && j + 8 <= fast ? load_eight(p, i * slow_stride + j, dtype) : load_line(p, i * slow_stride, fast_stride, j, fast, dtype);
 #pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        even = fma((double)v[e], (double)v[e], even);
-        odd = fma((double)v[e + 1], (double)v[e + 1], odd);
-      }
-    } else {
-      for (int e = j; e < j + 8 && e < fast; ++e) {
-        const double v = (double)load_value(p, i * slow_stride + e * fast_stride, dtype);
-        even = fma(v, v, even);
-      }
+    for (int e = 0; e < 8; e += 2) {
+      even = fma((double)v[e], (double)v[e], even);
+      odd = fma((double)v[e + 1], (double)v[e + 1], odd);
     }
   }
   double sum = even + odd;
@@ -94,14 +87,9 @@ __global__ __launch_bounds__(256) void k_lay_out(LayOut p) {
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     const int s = s0 + q * 32 + tid / 8, f = f0 + tid % 8 * 8;
-    v[q] = float8v{};
-    if (s < p.slow && p.wide && f + 8 <= p.fast) {
-      v[q] = load_eight(in, s * p.slow_stride + f, p.dtype);
-    } else if (s < p.slow) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (f + e < p.fast) v[q][e] = load_value(in, s * p.slow_stride + (f + e) * p.fast_stride, p.dtype);
-    }
+    const int64_t line = (s < p.slow ? s : p.slow - 1) * p.slow_stride;
+    v[q] = p.wide && f + 8 <= p.fast ? load_eight(in, line + f, p.dtype) : load_line(in, line, p.fast_stride, f, p.fast, p.dtype);
+    if (s >= p.slow) v[q] = float8v{};
   }
   double sum = 0.0;
   for (int i = tid; i < p.shares; i += 256) sum += p.squares[(int64_t)z * p.shares + i];

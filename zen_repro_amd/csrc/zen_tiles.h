@@ -247,6 +247,33 @@ __device__ __forceinline__ float8v load_eight(const char *p, int64_t i, int dtyp
   return widen(*reinterpret_cast<const half8v *>(p + i * 2));
 }
 
+// `of(e)`-th elements for e below N, all on their way together: no branch but the one on the type, which stands around them.
+template <int N, class T, class At>
+__device__ __forceinline__ void load_these(const char *p, float (&v)[N], At of) {
+  T raw[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) raw[e] = reinterpret_cast<const T *>(p)[of(e)];
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] = (float)raw[e];
+}
+
+template <int N, class At>
+__device__ __forceinline__ void load_values(const char *p, int dtype, float (&v)[N], At of) {
+  if (dtype == ZEN_F32) load_these<N, float>(p, v, of);
+  else if (dtype == ZEN_BF16) load_these<N, __bf16>(p, v, of);
+  else load_these<N, _Float16>(p, v, of);
+}
+
+// Elements j to j + 7 of a line of n a stride apart, zeros behind its end.
+__device__ __forceinline__ float8v load_line(const char *p, int64_t line, int64_t stride, int j, int n, int dtype) {
+  float v[8];
+  load_values(p, dtype, v, [&](int e) { return line + (j + e < n ? j + e : n - 1) * stride; });
+  float8v out;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) out[e] = j + e < n ? v[e] : 0.f;
+  return out;
+}
+
 __device__ __forceinline__ void store_eight(char *p, int64_t i, int dtype, float8v v) {
   if (dtype == ZEN_F32) *reinterpret_cast<float8v *>(p + i * 4) = v;
   else if (dtype == ZEN_BF16) *reinterpret_cast<bf8 *>(p + i * 2) = __builtin_convertvector(v, bf8);
@@ -362,28 +389,37 @@ struct OutEpilogue {
     for (int turn = 0; turn < turns; ++turn) {
       const bool down = (out_rs < out_cs) != (turn == 1);  // neighbouring lanes are neighbours of a column
       for (int base = lane; base < 32 * COLS; base += 64 * AT) {
-        float v[AT];
-        int64_t to[AT];
+        float v[AT], read[AT];
+        int i[AT], j[AT];
         bool there[AT];
 #pragma unroll
         for (int u = 0; u < AT; ++u) {  // no branches: what lies beyond the matrix reads its last row or column
           const int at = base + u * 64;
           const int di = down ? at & 31 : at / COLS, dj = down ? at >> 5 : at % COLS;
           there[u] = i0 + di < rows && j0 + dj < cols;
-          const int i = i0 + di < rows ? i0 + di : rows - 1, j = j0 + dj < cols ? j0 + dj : cols - 1;
-          const int64_t to_i = turn ? j : i, to_j = turn ? i : j;
+          i[u] = i0 + di < rows ? i0 + di : rows - 1;
+          j[u] = j0 + dj < cols ? j0 + dj : cols - 1;
           v[u] = alpha * sums[di * T::row + dj];
-          if (x) {
-            const int64_t from = z * x_batch + (int64_t)i * x_ld + j;
-            v[u] += beta * ((float)x[from] + (float)x_low[from]);
-          }
-          v[u] *= gain;
-          if (r) v[u] += keep * load_value(r, to_i * res_rs + to_j * res_cs, res_type);
-          to[u] = to_i * out_rs + to_j * out_cs;
+        }
+        if (x) {
+          const auto from = [&](int u) { return z * x_batch + (int64_t)i[u] * x_ld + j[u]; };
+          load_these<AT, _Float16>(reinterpret_cast<const char *>(x), read, from);
+#pragma unroll
+          for (int u = 0; u < AT; ++u) v[u] += beta * read[u];
+          load_these<AT, _Float16>(reinterpret_cast<const char *>(x_low), read, from);
+#pragma unroll
+          for (int u = 0; u < AT; ++u) v[u] += beta * read[u];
+        }
+#pragma unroll
+        for (int u = 0; u < AT; ++u) v[u] *= gain;
+        if (r) {
+          load_values(r, res_type, read, [&](int u) { return (turn ? j[u] : i[u]) * res_rs + (turn ? i[u] : j[u]) * res_cs; });
+#pragma unroll
+          for (int u = 0; u < AT; ++u) v[u] += keep * read[u];
         }
 #pragma unroll
         for (int u = 0; u < AT; ++u)
-          if (there[u]) store_value(o, to[u], out_type, v[u]);
+          if (there[u]) store_value(o, (turn ? j[u] : i[u]) * out_rs + (turn ? i[u] : j[u]) * out_cs, out_type, v[u]);
       }
     }
   }
