@@ -750,7 +750,8 @@ int zen_product(const zen_product_args *args);
  * and out = X (weights null), or, applied to weights in place,  W = keep * W - gain * X.
  * updates, outs and weights are HOST arrays of device addresses.  Types: any of the three for each.  `precise`: every operand is
  * held in 22 bits (two of fp16) and a product is three (results to fp32's accuracy); else the operands of the
- * products are fp16 and X is carried from step to step in 22 bits.
+ * products are fp16 and X is carried from step to step in 22 bits: results are off by less than bf16 rounds where the smaller side
+ * is at least 64, by up to three times that for very small matrices.
  * An update of zeros gives zeros.  outs may be the updates themselves (same type and strides), else nothing overlaps.
  */
 typedef struct zen_orthogonal_args {

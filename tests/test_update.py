@@ -783,3 +783,23 @@ def test_muon_behind_the_hook():
             # step; it is amplified by at most a^5 along the weakest directions, 2^-8 2^-8 485 of the whole
             limit = 0.02 * scale * (room + 485 * 2.0 ** -16) * o.norm() + 4 * U[F32] * before[i].norm()
             assert (p.detach().double().cpu() - want).norm() <= limit
+
+
+# ------------------------------------------------- precision of bf16 results
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,kind", [
+    (1, 1, "gauss"), (3, 2, "gauss"), (2, 50, "strong"), (8, 500, "gauss"), (16, 400, "gauss"), (48, 48, "gauss"), (48, 3000, "gauss"),
+    (3000, 48, "gauss"), (63, 64, "gauss"), (64, 64, "gauss"), (64, 1000, "gauss"), (100, 2000, "gauss"), (3000, 100, "strong"),
+    (128, 1023, "gauss"), (192, 6000, "gauss"), (255, 500, "strong"), (384, 6000, "gauss"), (500, 640, "gauss")])
+def test_orthogonal_part_for_bf16_is_off_by_less_than_bf16_rounds(m, n, kind):
+    """What fewer bits in the products do to a bf16 result is to stay below what the result's own rounding does, whatever the
+    shape.  Seen before that rounding: as what an fp32 weight of zeros gets."""
+    u = update_like(m, n, 300, kind)
+    want = newton_schulz(u, eps=0.0)
+    part = torch.zeros(m, n, device="cuda")
+    zen.orthogonal_step(part, u, 1.0, scale=-1.0, eps=0.0, precision=BF16)
+    # (of fewer than a hundred values the rounding may be any: a quarter of bf16's step is what it is by the mean)
+    room = off(want.to(BF16), want) if m * n >= 100 else U[BF16] / 4
+    assert off(part, want) <= room

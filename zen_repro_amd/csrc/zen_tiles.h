@@ -325,12 +325,18 @@ struct OutEpilogue {
   float alpha, beta, gain, keep;
   const _Float16 *x, *x_low;  // null: none (and no mirror image where there is one)
   int64_t x_ld, x_batch;
+  const float *row_low;       // with x: what rounding left over of the left operand's diagonal, a row's times alpha joins beta (null: none)
+  int64_t low_batch;
   int rows, cols;
   MatList out, res;             // res: listed < 0 for none
   int64_t out_rs, out_cs, res_rs, res_cs;
   int out_type, res_type;
   int lines;                    // 1: rows of out and res are contiguous and begin at multiples of 16 bytes; 2: columns
                                 // do (and there is no mirror image); 0: neither
+
+  __device__ __forceinline__ float beta_of(int z, int i) const {
+    return row_low ? fmaf(alpha, row_low[z * low_batch + i], beta) : beta;
+  }
 
   template <int COLS, int AT>
   __device__ __forceinline__ void block(int z, int i0, int j0, float *sums, bool mirror, int lane) const {
@@ -347,7 +353,7 @@ struct OutEpilogue {
         const int i = i0 + di, j = j0 + dj;
         if (x) {
           const int64_t at = z * x_batch + (int64_t)i * x_ld + j;
-          v += beta * (widen(*reinterpret_cast<const half8v *>(x + at)) + widen(*reinterpret_cast<const half8v *>(x_low + at)));
+          v += beta_of(z, i) * (widen(*reinterpret_cast<const half8v *>(x + at)) + widen(*reinterpret_cast<const half8v *>(x_low + at)));
         }
         v *= gain;
         if (lines == 2) {
@@ -403,12 +409,11 @@ struct OutEpilogue {
         }
         if (x) {
           const auto from = [&](int u) { return z * x_batch + (int64_t)i[u] * x_ld + j[u]; };
+          float low[AT];
           load_these<AT, _Float16>(reinterpret_cast<const char *>(x), read, from);
+          load_these<AT, _Float16>(reinterpret_cast<const char *>(x_low), low, from);
 #pragma unroll
-          for (int u = 0; u < AT; ++u) v[u] += beta * read[u];
-          load_these<AT, _Float16>(reinterpret_cast<const char *>(x_low), read, from);
-#pragma unroll
-          for (int u = 0; u < AT; ++u) v[u] += beta * read[u];
+          for (int u = 0; u < AT; ++u) v[u] += beta_of(z, i[u]) * (read[u] + low[u]);
         }
 #pragma unroll
         for (int u = 0; u < AT; ++u) v[u] *= gain;
@@ -425,8 +430,18 @@ struct OutEpilogue {
   }
 };
 
-// What goes back to a workspace: d = alpha * acc + beta * (c + c') + diag on the diagonal, in one or two times 16 bits, and
-// (t not null) its transpose beside it.  Rows and columns are multiples of 64.
+// What goes back to a workspace, of the three products of a step:
+//   kGram    d = alpha acc
+//   kSquare  d = alpha acc + beta c + diag on the diagonal, where acc is c c
+//   kApply   d = alpha acc + beta (c + c'), its transpose t beside it, where acc is P c
+// in 16 bits, for kApply in twice 16.  Rows and columns are multiples of 64.
+// HALVES: every operand has its left-over (c', d', t') in 16 bits.  Otherwise the diagonals of what kGram and kSquare write are kept
+// whole: their entries are often nearly equal, so that rounding takes all of them the same way and scales the whole product (384
+// x 6000: results off by 1.4e-3, 0.6e-3 with whole diagonals).  What their rounding leaves over goes to `low` and is made good where
+// the matrix is used, for a number an element.
+enum Keep { kGram, kSquare, kApply };
+
+template <Keep WHAT, bool HALVES>
 struct KeepEpilogue {
   float alpha, beta, diag;
   int rows, cols;
@@ -434,32 +449,68 @@ struct KeepEpilogue {
   const _Float16 *c, *c_low;
   _Float16 *d, *d_low, *t, *t_low;
   int64_t ld, batch, t_ld, t_batch;  // c lies as d does
+  float *low;             // kGram, kSquare: of d's diagonal
+  const float *from_low;  // kSquare: of c's diagonal; kApply: of P's
+  int64_t low_batch;      // of both
 
+  template <bool LOW>
   static __device__ __forceinline__ void store(_Float16 *p, _Float16 *low, int64_t at, float8v v) {
     const half8v h = __builtin_convertvector(v, half8v);
     *reinterpret_cast<half8v *>(p + at) = h;
-    if (low) *reinterpret_cast<half8v *>(low + at) = __builtin_convertvector(v - widen(h), half8v);
+    if constexpr (LOW) *reinterpret_cast<half8v *>(low + at) = __builtin_convertvector(v - widen(h), half8v);
   }
 
   template <int COLS, int AT>
   __device__ __forceinline__ void block(int z, int i0, int j0, float *sums, bool mirror, int lane) const {
     using T = Stage<COLS>;
+    constexpr bool kWhole = !HALVES && WHAT != kApply;
     if (i0 >= rows || j0 >= cols) return;
-    const bool turned = mirror || t;
+    const bool turned = mirror || WHAT == kApply;
+    const float *l = HALVES || WHAT == kGram ? nullptr : from_low + z * low_batch;
+    float8v across = {};
+    if constexpr (!HALVES && WHAT == kSquare) {
+      int di, dj;
+      T::of_row(0, lane, di, dj);  // a lane's columns are the same in every turn
+      across = *reinterpret_cast<const float8v *>(l + j0 + dj);
+    }
 #pragma unroll
     for (int turn = 0; turn < T::turns; ++turn) {
       int di, dj;
       T::of_row(turn, lane, di, dj);
       const int i = i0 + di, j = j0 + dj;
       const int64_t at = z * batch + (int64_t)i * ld + j;
-      float8v v = alpha * T::row_sums(sums, di, dj);
-      if (c) v += beta * widen(*reinterpret_cast<const half8v *>(c + at));
-      if (c_low) v += beta * widen(*reinterpret_cast<const half8v *>(c_low + at));
-      if (diag != 0.f && i >= j && i < j + 8 && i < diag_n) {
+      const bool crossed = i >= j && i < j + 8;  // by the diagonal
+      float8v v = T::row_sums(sums, di, dj);
+      if constexpr (WHAT != kGram) {
+        float8v own = widen(*reinterpret_cast<const half8v *>(c + at));
+        float times = beta;
+        if constexpr (!HALVES && WHAT == kApply) times = fmaf(alpha, l[i], beta);  // (P + l) c for a diagonal l
+        if constexpr (!HALVES && WHAT == kSquare) {  // (c + l)(c + l): l l is beyond fp32's last bit
+          const float mine = l[i];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += i == j + e ? diag : 0.f;
+          for (int e = 0; e < 8; ++e) {
+            v[e] = fmaf(own[e], mine + across[e], v[e]);
+            own[e] += i == j + e ? mine : 0.f;
+          }
+        }
+        if constexpr (HALVES || WHAT == kApply) own += widen(*reinterpret_cast<const half8v *>(c_low + at));
+        v = alpha * v + times * own;
+      } else {
+        v *= alpha;
       }
-      store(d, d_low, at, v);
+      if constexpr (WHAT == kSquare) {
+        if (diag != 0.f && crossed && i < diag_n) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += i == j + e ? diag : 0.f;
+        }
+      }
+      store<HALVES || WHAT == kApply>(d, d_low, at, v);
+      if (kWhole && crossed) {
+        float left = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) left += i == j + e ? v[e] - (float)(_Float16)v[e] : 0.f;
+        low[z * low_batch + i] = left;
+      }
       if (turned) T::put_row(sums, di, dj, v);
     }
     if (!turned) return;
@@ -470,7 +521,7 @@ struct KeepEpilogue {
     for (int turn = 0; turn < T::turns; ++turn) {
       int di, dj;
       T::of_column(turn, lane, di, dj);
-      store(to, to_low, from + (int64_t)(j0 + dj) * to_ld + i0 + di, T::column_sums(sums, di, dj));
+      store<HALVES>(to, to_low, from + (int64_t)(j0 + dj) * to_ld + i0 + di, T::column_sums(sums, di, dj));
     }
   }
 };

@@ -134,7 +134,8 @@ def orthogonalize(update, steps=5, coefficients=COEFFICIENTS, eps=1e-7, dtype=No
     update  a matrix, a stack (3-D) or a list of matrices of one shape; fp32, bf16 or fp16, any strides.  Many small matrices
             are quicker in one call than one by one
     dtype   the result's type (default: the update's).  It decides the precision: for bf16 the products' operands are
-            fp16, for fp32 and fp16 they have 22 bits (three products of fp16 each); the iterate has 22 bits
+            fp16 where the smaller side is at least 64 (off by less than the result's own rounding then), below
+            that, and for fp32 and fp16, they have 22 bits (three products of fp16 each); the iterate has 22 bits
     out     where the result goes, of the update's shape (a list for a list); may be the update itself"""
     updates = _matrices(update, "update")
     listed = isinstance(update, (list, tuple))
