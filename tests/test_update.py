@@ -803,3 +803,26 @@ def test_orthogonal_part_for_bf16_is_off_by_less_than_bf16_rounds(m, n, kind):
     # (of fewer than a hundred values the rounding may be any: a quarter of bf16's step is what it is by the mean)
     room = off(want.to(BF16), want) if m * n >= 100 else U[BF16] / 4
     assert off(part, want) <= room
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -10, 2.0 ** -20, 2.0 ** -30])  # of gradients with an RMS of 1e-3
+@pytest.mark.parametrize("precision", [F32, BF16, F16])
+def test_muon_steps_alike_whatever_the_gradients_size(precision, size):
+    g, before = update_like(96, 80, 310), normal((96, 80), 311, F32, 0.02)
+    p = torch.nn.Parameter(before.clone())
+    opt = zen.Muon([p], lr=0.02, eps=0.0, precision=precision)
+    p.grad = g * size
+    opt.step()
+    u = (g.double() + MU * g.double()).float()
+    if precision == BF16:
+        want = newton_schulz(u.to(BF16), eps=0.0)
+        # the products' roundings stay below bf16's own; an update rounded the other way, as in test_muon_behind_the_hook
+        room = off(want.to(BF16), want) + 485 * 2.0 ** -16
+    else:
+        want = newton_schulz(u, eps=0.0)
+        plain = newton_schulz_fp32(u.T, eps=0.0).T
+        room = 4 * max(off(plain, want), 4 * U[F32])  # as in room_of
+    part = 0.02 * math.sqrt(96 / 80)
+    limit = part * room * want.norm() + 4 * U[F32] * before.double().norm().item()
+    assert (p.detach().double().cpu() - (before.double().cpu() - part * want)).norm() <= limit

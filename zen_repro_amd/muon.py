@@ -18,8 +18,9 @@ class Muon(torch.optim.Optimizer):
     momentum, nesterov, weight_decay, steps, coefficients, eps   see momentum_update and orthogonal_step
     match_rms     a number r: scale = r * sqrt(max(rows, cols)), which gives every update's elements an RMS of about
                   r * lr whatever the matrix' shape; None: scale = sqrt(max(1, rows / cols))
-    precision     of the orthogonalisation (see orthogonal_step), and the type in which the momentum hands the update
-                  on (default bfloat16; float32 for fp32's accuracy throughout)
+    precision     of the orthogonalisation (see orthogonal_step; default bfloat16).  The momentum hands the update on in
+                  bfloat16 for bfloat16, else in float32: only its direction counts, and a small gradient is below
+                  fp16's range
     The momentum is kept in fp32.  Parameters of one shape go through the orthogonalisation together."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,
@@ -63,8 +64,9 @@ class Muon(torch.optim.Optimizer):
                 state = self.state[p]
                 if "momentum" not in state:
                     state["momentum"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                handed_on = torch.bfloat16 if group["precision"] == torch.bfloat16 else torch.float32
                 u = momentum_update(state["momentum"], p.grad.contiguous(), group["momentum"], group["nesterov"],
-                                    dtype=group["precision"])
+                                    dtype=handed_on)
                 key = (p.shape, p.dtype, p.device)
                 waiting = alike.setdefault(key, ([], []))
                 waiting[0].append(p)
