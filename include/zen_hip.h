@@ -705,7 +705,8 @@ int zen_momentum(void *momentum, int momentum_dtype, const void *grad, int grad_
  * counts; counts (null: none) is a HOST array of device addresses of int64 counts (or null), of which the smaller of
  * count and length holds.  All lists have one index type (idx64) and one value type.  n < 2^31.  Every index once to a list; an
  * index that several lists hold gets their values in the order of the lists.  An index outside [0, n), or one that is not larger than
- * its list's last one, sets ZEN_STAT_BAD_INDEX; then neither momentum nor update is written.
+ * its list's last one, sets ZEN_STAT_BAD_INDEX; then neither momentum nor update is written.  Nor are they where `*status` is not
+ * zero beforehand: it may be the status of the call that made the lists (zen_merge), whose answer then need not be waited for.
  */
 #define ZEN_MOMENTUM_LISTS_MOST 64
 size_t zen_momentum_lists_workspace(int64_t n, int lists);

@@ -826,3 +826,53 @@ def test_muon_steps_alike_whatever_the_gradients_size(precision, size):
     part = 0.02 * math.sqrt(96 / 80)
     limit = part * room * want.norm() + 4 * U[F32] * before.double().norm().item()
     assert (p.detach().double().cpu() - (before.double().cpu() - part * want)).norm() <= limit
+
+
+@pytest.mark.gpu
+def test_lists_of_a_call_that_failed_are_not_taken():
+    """The status of the call that made the lists goes along, unseen: whatever it says, nothing is written."""
+    n = 6000
+    (idx, val), = some_lists(n, [900], 400)
+    want = dense_of([(idx, val)], n)
+    for bits in (_lib.STAT_RETRY, _lib.STAT_CAPACITY, _lib.STAT_INTERNAL, _lib.STAT_BAD_INDEX, _lib.STAT_SERIAL_OVERFLOW, 0):
+        before = normal(n, 401)
+        m, out = before.clone(), torch.full((n,), 5.0, device="cuda")
+        status = torch.tensor([bits], dtype=torch.int32, device="cuda")
+        u, got = zen.momentum_update_sparse(m, idx, val, out=out, status=status)
+        assert got is status and u is out and got.item() == bits
+        if bits:
+            assert torch.equal(m, before) and out.eq(5.0).all()
+        else:
+            momentum_check(before, m, u, want[0], True, U[F32] * want[1])
+    # what this call finds goes into the word
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    _, got = zen.momentum_update_sparse(m, torch.tensor([5, 5], dtype=torch.int32, device="cuda"), val[:2], status=status)
+    assert got is status and status.item() == _lib.STAT_BAD_INDEX
+    for wrong, error in ((status.long(), TypeError), (torch.zeros(2, dtype=torch.int32, device="cuda"), ValueError),
+                         (status.cpu(), ValueError), (idx[:1], ValueError)):
+        with pytest.raises(error):
+            zen.momentum_update_sparse(m, idx, val, status=wrong)
+
+
+@pytest.mark.gpu
+def test_a_merge_that_is_declined_does_not_reach_the_momentum():
+    """Entries piled on one key make the merge's fast mode decline, its lists unspecified: its status keeps them out of the momentum
+    without a wait in between."""
+    n = 1 << 20
+    idx = torch.cat([torch.full((100000,), 12345), torch.randint(n, (50000,), generator=torch.Generator().manual_seed(1))]).int().cuda()
+    val = normal(idx.numel(), 410)
+    lba = zen.LoadBalanceAllreduce(zen.LocalGroup(4), None, None)
+    before = normal(n, 411)
+    for mode, declined in ((_lib.MODE_FAST, True), (_lib.MODE_GENERAL, False)):
+        m = before.clone()
+        mi, mv, count, status = lba.merge_sparse_flat(idx, val, n, mode=mode)
+        u, status = zen.momentum_update_sparse(m, mi, mv, mu=0.5, nesterov=False, counts=count, status=status)
+        if declined:
+            assert status.item() & _lib.STAT_RETRY and torch.equal(m, before)
+            lba.reset_merge_workspace(m.device)
+        else:
+            assert status.item() == 0
+            wi, wv = lba.merge_sparse(idx, val, n)
+            want = before * 0.5
+            want[wi] += wv
+            assert torch.equal(m, want) and torch.equal(u, want)  # halves are exact, one rounding each

@@ -435,11 +435,12 @@ py::tuple momentum(const py::object &fn, const Tensor &momentum, const Tensor &g
   return py::make_tuple(rc, out);
 }
 
-// counts: none, one tensor (an element to a list), or one tensor or none to a list
+// counts: none, one tensor (an element to a list), or one tensor or none to a list; before: the status word of the call that made the lists
 py::tuple momentum_lists(const py::object &fn, Zeros &zeros, const Tensor &momentum, const std::vector<Tensor> &indices,
                          const std::vector<Tensor> &values, double mu, bool nesterov, const std::optional<Tensor> &counted,
                          const std::optional<std::vector<std::optional<Tensor>>> &counts, const Dtype &dtype,
-                         const std::optional<Tensor> &given, const py::object &workspace, int64_t stream) {
+                         const std::optional<Tensor> &given, const std::optional<Tensor> &before, const py::object &workspace,
+                         int64_t stream) {
   const size_t lists = indices.size();
   if (lists < 1 || lists > ZEN_MOMENTUM_LISTS_MOST || values.size() != lists)
     throw py::value_error("1 to " + std::to_string(ZEN_MOMENTUM_LISTS_MOST) + " lists, as many of indices as of values: got " +
@@ -487,7 +488,16 @@ py::tuple momentum_lists(const py::object &fn, Zeros &zeros, const Tensor &momen
         count[l] = address(*(*counts)[l]);
       }
   }
-  const Tensor status = made([&] { return zeros.status(momentum, stream); });
+  if (before) {
+    on_one_device(momentum, *before);
+    if (before->scalar_type() != at::kInt) throw py::type_error("a status is int32");
+    if (before->numel() != 1) throw py::value_error("a status is one element");
+    apart(*before);
+    const auto from = [&](const Tensor &t) { return overlap(*before, t); };
+    if (std::any_of(indices.begin(), indices.end(), from) || std::any_of(values.begin(), values.end(), from))
+      throw py::value_error("momentum_update_sparse: the status overlaps a list");
+  }
+  const Tensor status = before ? *before : made([&] { return zeros.status(momentum, stream); });
   const Lists i(indices), v(values);
   const py::object rc = fn(address(momentum), type_of(momentum, "momentum"), i.addresses(), index == at::kLong ? 1 : 0, v.addresses(),
                            code, i.counts(), reinterpret_cast<int64_t>(count.data()), lists, n, mu, nesterov ? 1 : 0, address(out),
@@ -495,6 +505,7 @@ py::tuple momentum_lists(const py::object &fn, Zeros &zeros, const Tensor &momen
                            workspace.is_none() ? 0 : workspace.cast<Tensor>().numel(), address(status), stream);
   written(momentum);
   written(out);
+  if (before) written(status);
   return py::make_tuple(rc, out, status);
 }
 

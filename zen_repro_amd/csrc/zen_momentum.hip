@@ -133,7 +133,7 @@ __global__ __launch_bounds__(kBlock) void k_momentum_lists(M *momentum, Lists li
                                                            uint32_t tiles, const uint32_t *__restrict__ marks, float mu,
                                                            bool nesterov, U *update, const int32_t *status) {
   __shared__ float s_sum[kBlock / 64][kTile];
-  if (*status & ZEN_STAT_BAD_INDEX) return;
+  if (*status) return;  // a list that is none, or the call that made the lists said so of them all
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t tile = blockIdx.x * (kBlock / 64) + (uint32_t)wave;
   if (tile >= tiles) return;

@@ -44,7 +44,7 @@ def momentum_update(momentum, grad, mu=0.95, nesterov=True, dtype=None, out=None
 
 
 def momentum_update_sparse(momentum, indices_tensors, values_tensors, mu=0.95, nesterov=True, counts=None, dtype=None,
-                           out=None):
+                           out=None, status=None):
     """momentum_update with the gradient as ascending lists of (index, value), zero elsewhere: what merge_sparse_flat
     returns, or every rank's list of the second exchange, without the dense tensor in between.  Returns (update,
     status int32[1]).
@@ -55,6 +55,8 @@ def momentum_update_sparse(momentum, indices_tensors, values_tensors, mu=0.95, n
     counts    how many entries of each list hold: None (all), an int64 tensor on the device (one element per list), or a list of
               such one-element tensors or None
     dtype     the update's type (default: the values')
+    status    the status of the call that made the lists (int32[1] on the device, as merge_sparse_flat returns it), where
+              nobody has looked at it yet.  If it is not zero, nothing is written; else what this call finds goes into it
     An index outside the momentum, or not larger than its list's last one, sets STAT_BAD_INDEX in the status: nothing is
     written then (the update's contents are whatever its memory held)."""
     indices = indices_tensors if isinstance(indices_tensors, (list, tuple)) else [indices_tensors]
@@ -67,7 +69,7 @@ def momentum_update_sparse(momentum, indices_tensors, values_tensors, mu=0.95, n
     if momentum.is_cuda:
         ws = _workspace(momentum.device, L.zen_momentum_lists_workspace(momentum.numel(), len(indices)))
     rc, out, status = _called(momentum, _lib.host.momentum_lists, L.zen_momentum_lists, _lib.zeros.native(), momentum, indices,
-                              values, mu, nesterov, counted, counts, dtype, out, ws)
+                              values, mu, nesterov, counted, counts, dtype, out, status, ws)
     if rc:
         _lib.check(rc, "momentum_update_sparse")
     return out, status
