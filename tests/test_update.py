@@ -876,3 +876,35 @@ def test_a_merge_that_is_declined_does_not_reach_the_momentum():
             want = before * 0.5
             want[wi] += wv
             assert torch.equal(m, want) and torch.equal(u, want)  # halves are exact, one rounding each
+
+
+@pytest.mark.gpu
+def test_ranks_stay_alike_from_the_exchange_to_the_weights():
+    """Four ranks: buckets to their partitions, each partition merged where it belongs, all lists to every rank, momentum and
+    weights from them: every rank ends with the update of the whole gradient."""
+    rows, cols, ranks = 96, 160, 4
+    n = rows * cols
+    grads = [torch.zeros(n, device="cuda").index_put_((i.long(),), v) for i, v in some_lists(n, [900] * ranks, 420, shared=60)]
+    lba = [zen.LoadBalanceAllreduce(zen.LocalGroup(ranks, r), None, None) for r in range(ranks)]
+    sent = [lba[r].tensor_partition.load_balance(g) for r, g in enumerate(grads)]
+    merged = [lba[r].merge_rounded([s[0][r].clone() for s in sent], [s[1][r].clone() for s in sent], n, F32) for r in range(ranks)]
+    total = torch.stack(grads).double().sum(0)
+    size = torch.stack(grads).double().abs().sum(0)
+    total[0] = size[0] = 0.0  # the partition's tables have no place for index 0, as the reference's: it is not sent
+    before = normal((rows, cols), 421, F32, 0.02)
+    results = []
+    for r in range(ranks):
+        m, w = torch.zeros(rows, cols, device="cuda"), before.clone()
+        u, status = zen.momentum_update_sparse(m, [i for i, _ in merged], [v for _, v in merged])
+        assert status.item() == 0
+        zen.orthogonal_step(w, u, 0.1)
+        momentum_check(torch.zeros(n, device="cuda"), m.view(-1), u.view(-1), total, True, ranks * U[F32] * size)
+        results.append((m, u, w))
+    for r in range(1, ranks):
+        assert all(torch.equal(a, b) for a, b in zip(results[0], results[r]))
+    o, room = room_of(results[0][1], F32)
+    want = before.double().cpu() - 0.1 * o
+    assert (results[0][2].double().cpu() - want).norm() <= 0.1 * room * o.norm() + 4 * U[F32] * want.norm()
+    # one rank's merge alone is a part of it: the indices that its partition owns
+    parts = [set(i.tolist()) for i, _ in merged]
+    assert sum(len(p) for p in parts) == len(set().union(*parts)) == int((total != 0).sum())

@@ -13,7 +13,8 @@ class Muon(torch.optim.Optimizer):
     """weight = (1 - lr * weight_decay) * weight - lr * scale * O(u), with u the (Nesterov) momentum of the gradient and O its
     orthogonalisation.
 
-    params        parameters with two dimensions (others: any other optimiser), fp32 or bf16 or fp16
+    params        the layers' matrices: parameters with two dimensions, fp32 or bf16 or fp16 (embeddings, the output head and
+                  everything else: any other optimiser)
     lr            about the RMS that an update's elements get, relative to `scale`
     momentum, nesterov, weight_decay, steps, coefficients, eps   see momentum_update and orthogonal_step
     match_rms     a number r: scale = r * sqrt(max(rows, cols)), which gives every update's elements an RMS of about

@@ -45,9 +45,10 @@ def momentum_update(momentum, grad, mu=0.95, nesterov=True, dtype=None, out=None
 
 def momentum_update_sparse(momentum, indices_tensors, values_tensors, mu=0.95, nesterov=True, counts=None, dtype=None,
                            out=None, status=None):
-    """momentum_update with the gradient as ascending lists of (index, value), zero elsewhere: what merge_sparse_flat
-    returns, or every rank's list of the second exchange, without the dense tensor in between.  Returns (update,
-    status int32[1]).
+    """momentum_update with the gradient as ascending lists of (index, value), zero elsewhere, without the dense tensor in
+    between: every rank's list of the second exchange (merge_rounded's result of each, gathered).  A rank's own merge
+    (merge_rounded, merge_sparse_flat) is the sum over its partition alone, a part of the gradient only.  Returns
+    (update, status int32[1]).
 
     indices_tensors, values_tensors   a tensor each, or a list of up to 64; int32 or int64 indices into the flat momentum,
               every index once to a list; fp32, bf16 or fp16 values.  An index that several lists hold gets its values
