@@ -721,7 +721,7 @@ int zen_momentum_lists(void *momentum, int momentum_dtype, const void *const *id
  * where one of the two is 1 and addresses and the other stride are multiples of 16 bytes (for b with b_rs == 1, and a with
  * a_cs == 1, k too), they are read as they lie, else they are laid out in the workspace first.  c (null: none) and out: any
  * strides, ZEN_F32, ZEN_BF16 or ZEN_F16; out may be c itself (the same addresses and strides), else it overlaps nothing.
- * symmetric: the caller vouches that a b is (m == n): half of it is computed and mirrored.  k is at most 2^21.
+ * symmetric: the caller vouches that a b is (m == n): half of it is computed and mirrored.  k is at most 2^21, batch 65535.
  */
 typedef struct zen_product_args {
   const void *a;
@@ -753,7 +753,7 @@ int zen_product(const zen_product_args *args);
  * held in 22 bits (two of fp16) and a product is three (results to fp32's accuracy); else the operands of the
  * products are fp16 and X is carried from step to step in 22 bits: results are off by less than bf16 rounds where the smaller side
  * is at least 64, by up to three times that for very small matrices.
- * An update of zeros gives zeros.  outs may be the updates themselves (same type and strides), else nothing overlaps.
+ * rows and cols are at most 2^21.  An update of zeros gives zeros.  outs may be the updates themselves (same type and strides), else nothing overlaps.
  */
 typedef struct zen_orthogonal_args {
   const void *const *updates;

@@ -908,3 +908,23 @@ def test_ranks_stay_alike_from_the_exchange_to_the_weights():
     # one rank's merge alone is a part of it: the indices that its partition owns
     parts = [set(i.tolist()) for i, _ in merged]
     assert sum(len(p) for p in parts) == len(set().union(*parts)) == int((total != 0).sum())
+
+
+@pytest.mark.gpu
+def test_limits_are_named_before_memory_is_asked_for():
+    """Views of one element: nothing of these sizes is there."""
+    one = torch.zeros(1, 1, 1, device="cuda")
+    half = one.to(BF16)
+    side, deep = (1 << 21) + 1, (1 << 21) + 8
+    for call, name in [
+            (lambda: zen.orthogonalize(one[0].expand(side, 2)), "2^21"), (lambda: zen.orthogonalize(one[0].expand(1, side)), "2^21"),
+            (lambda: zen.orthogonal_step(torch.zeros(2, side, device="cuda"), one[0].expand(2, side), 0.1), "2^21"),
+            (lambda: zen.product(half[0].expand(1, deep), half[0].expand(deep, 1)), "2^21"),
+            (lambda: zen.product(half.expand(4000, 500, deep), half.expand(4000, deep, 1)), "2^21"),  # 8 TB if it were laid out
+            (lambda: zen.product(half.expand(65536, 1, 8), half.expand(65536, 8, 1)), "65535")]:
+        with pytest.raises(ValueError) as e:
+            call()
+        assert name in str(e.value)
+    assert zen.product(half.expand(65535, 1, 8), half.expand(65535, 8, 1)).eq(0).all()
+    assert zen.orthogonalize(one[0].expand(1 << 21, 1)).eq(0).all()
+    assert zen.product(half[0].expand(1, 1 << 21), half[0].expand(1 << 21, 1)).eq(0).all()

@@ -658,8 +658,11 @@ py::object orthogonal(const py::object &fn, const py::object &bytes_of, const py
     p.out_rs = strides[2];
     p.out_cs = strides[3];
     p.workspace_bytes = bytes_of(p.rows, p.cols, p.count, p.precise).cast<size_t>();
-    const Tensor ws = room(p.workspace_bytes).cast<Tensor>();
-    p.workspace = ws.data_ptr();
+    Tensor ws;
+    if (p.workspace_bytes) {  // none: the call is refused
+      ws = room(p.workspace_bytes).cast<Tensor>();
+      p.workspace = ws.data_ptr();
+    }
     rc = fn(reinterpret_cast<int64_t>(&p));
     if (rc.cast<int>() != ZEN_OK) break;
   }

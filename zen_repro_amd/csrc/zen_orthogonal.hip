@@ -329,8 +329,8 @@ int zen_orthogonal(const zen_orthogonal_args *p) {
   if (!p) return fail(ZEN_EINVAL, "zen_orthogonal: null pointer");
   const auto known = [](int t) { return t == ZEN_F32 || t == ZEN_BF16 || t == ZEN_F16; };
   if (!known(p->update_dtype) || !known(p->out_dtype)) return fail(ZEN_EINVAL, "zen_orthogonal: types are fp32, bf16 or fp16");
-  if (p->rows < 0 || p->cols < 0 || p->count < 0 || p->rows > kMostSide || p->cols > kMostSide)
-    return fail(ZEN_EINVAL, "zen_orthogonal: a size is out of range");
+  if (p->rows < 0 || p->cols < 0 || p->count < 0) return fail(ZEN_EINVAL, "zen_orthogonal: a size is out of range");
+  if (p->rows > kMostSide || p->cols > kMostSide) return fail(ZEN_EINVAL, "zen_orthogonal: a side is at most 2^21");
   if (p->steps < 1) return fail(ZEN_EINVAL, "zen_orthogonal: at least one step");
   if (!(p->eps >= 0)) return fail(ZEN_EINVAL, "zen_orthogonal: eps is not negative");
   if (p->update_rs < 0 || p->update_cs < 0 || p->out_rs < 0 || p->out_cs < 0) return fail(ZEN_EINVAL, "zen_orthogonal: negative stride");

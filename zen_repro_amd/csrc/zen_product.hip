@@ -54,6 +54,8 @@ bool lay_out(Side &s, int64_t batches, Carver &cv, PackArgs &p) {
   return true;
 }
 
+constexpr int64_t kMostStack = 65535;
+
 bool known(int type) { return type == ZEN_F32 || type == ZEN_BF16 || type == ZEN_F16; }
 int64_t size_of(int type) { return type == ZEN_F32 ? 4 : 2; }
 
@@ -74,8 +76,10 @@ int lines(const void *p, int64_t rs, int64_t cs, int64_t batch, int type, int64_
 int check(const zen_product_args *p) {
   if (!p) return fail(ZEN_EINVAL, "zen_product: null pointer");
   const int64_t most = 0x7fffffffll - 1024;
-  if (p->m < 0 || p->n < 0 || p->k < 0 || p->batch < 0 || p->m > most || p->n > most || p->k > most || p->batch > 65535)
+  if (p->m < 0 || p->n < 0 || p->k < 0 || p->batch < 0 || p->m > most || p->n > most)
     return fail(ZEN_EINVAL, "zen_product: a size is out of range");
+  if (p->k > kMostLd) return fail(ZEN_EINVAL, "zen_product: k is at most 2^21");
+  if (p->batch > kMostStack) return fail(ZEN_EINVAL, "zen_product: at most 65535 matrices");
   if (p->dtype != ZEN_BF16 && p->dtype != ZEN_F16) return fail(ZEN_EINVAL, "zen_product: a and b are bf16 or fp16");
   if (!known(p->out_dtype) || (p->c && !known(p->c_dtype))) return fail(ZEN_EINVAL, "zen_product: c and out are fp32, bf16 or fp16");
   if (p->symmetric && p->m != p->n) return fail(ZEN_EINVAL, "zen_product: a symmetric result is square");
@@ -107,7 +111,6 @@ int zen_product(const zen_product_args *p) {
   if (const int rc = check(p)) return rc;
   if (p->m == 0 || p->n == 0 || p->batch == 0) return ZEN_OK;
   if (!p->out || (p->k > 0 && (!p->a || !p->b))) return fail(ZEN_EINVAL, "zen_product: null pointer");
-  if (p->k > kMostLd) return fail(ZEN_EINVAL, "zen_product: k is at most 2^21");
   const size_t need = zen_product_workspace(p);
   if (need && !p->workspace) return fail(ZEN_EINVAL, "zen_product: null pointer");
   if (p->workspace_bytes < need) return fail(ZEN_EWORKSPACE, "zen_product: workspace too small");

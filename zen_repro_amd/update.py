@@ -84,7 +84,7 @@ def product(a, b, residual=None, alpha=1.0, beta=1.0, symmetric=False, dtype=Non
 
     a, b       bf16 or fp16 matrices (m x k and k x n), or stacks of as many; any strides.  Where rows or columns are contiguous
                and begin at multiples of 16 bytes they are read as they lie (a transposed view costs nothing), else
-               laid out first.  k is at most 2^21
+               laid out first.  k is at most 2^21, a stack of 65535 matrices
     residual   m x n (or a stack), fp32, bf16 or fp16, any strides.  It is read whatever beta is: NaN in it stays NaN
     symmetric  the caller vouches that a @ b is symmetric (a matrix and its own transpose, powers of a symmetric
                matrix): half of it is computed and mirrored
@@ -134,8 +134,8 @@ def orthogonalize(update, steps=5, coefficients=COEFFICIENTS, eps=1e-7, dtype=No
     """The update with its singular values taken to about one: from X = U / (|U| + eps) (Frobenius norm), `steps` times
     X = a X + (b A + c A A) X with A = X X^T, on the side of the smaller dimension.  An update of zeros gives zeros.
 
-    update  a matrix, a stack (3-D) or a list of matrices of one shape; fp32, bf16 or fp16, any strides.  Many small matrices
-            are quicker in one call than one by one
+    update  a matrix, a stack (3-D) or a list of matrices of one shape; fp32, bf16 or fp16, any strides, rows and columns
+            up to 2^21.  Many small matrices are quicker in one call than one by one
     dtype   the result's type (default: the update's).  It decides the precision: for bf16 the products' operands are
             fp16 where the smaller side is at least 64 (off by less than the result's own rounding then), below
             that, and for fp32 and fp16, they have 22 bits (three products of fp16 each); the iterate has 22 bits
