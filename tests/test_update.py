@@ -928,3 +928,16 @@ def test_limits_are_named_before_memory_is_asked_for():
     assert zen.product(half.expand(65535, 1, 8), half.expand(65535, 8, 1)).eq(0).all()
     assert zen.orthogonalize(one[0].expand(1 << 21, 1)).eq(0).all()
     assert zen.product(half[0].expand(1, 1 << 21), half[0].expand(1 << 21, 1)).eq(0).all()
+
+
+def test_more_threads_than_a_launch_takes_are_refused(L):
+    """Nothing is launched or dereferenced: addresses are made up."""
+    one = ctypes.c_void_p(256)
+    most = (1 << 32) - 1  # threads
+    assert L.zen_momentum(one, 0, one, 0, most // 256 * 2048 + 1, 0.9, 1, one, 0, None) == _lib.EINVAL
+    side = 64 * 4097  # 4097 x 4097 tiles of 256 threads, or fewer and larger ones of as many to their elements
+    wide = dict(m=side * 8, n=side * 8, k=64, a_rs=64, b_rs=1, b_cs=64, out_rs=side * 8)
+    assert L.zen_product(product_args(**wide)) == _lib.EINVAL
+    # (k x n, every second element: laid out first)
+    assert L.zen_product(product_args(m=64, n=1 << 30, k=1 << 13, b_rs=2, b_cs=1 << 14, out_rs=1 << 30, workspace=256,
+                                      workspace_bytes=1 << 62)) == _lib.EINVAL

@@ -221,7 +221,7 @@ uint32_t tiles_of(int64_t n) { return (uint32_t)((n + kTile - 1) / kTile); }
 template <typename M, typename G, typename U>
 int dense(void *momentum, const void *grad, int64_t n, float mu, int nesterov, void *update, hipStream_t s) {
   const int64_t blocks = ceil_div(n, kBlock * 8);
-  if (blocks > 0x7fffffffll) return fail(ZEN_EINVAL, "zen_momentum: too many elements");
+  if (blocks > kMostThreads / kBlock) return fail(ZEN_EINVAL, "zen_momentum: too many elements");
   M *m = static_cast<M *>(momentum);
   const G *g = static_cast<const G *>(grad);
   U *u = static_cast<U *>(update);
@@ -318,7 +318,7 @@ int zen_momentum_lists(void *momentum, int momentum_dtype, const void *const *id
     all.first_block[l] = (uint32_t)blocks;
     blocks += (uint64_t)lengths[l] / (kBlock * kMarkPer) + 1;  // one more than the entries: the place behind the last one
   }
-  if (blocks > 0x7fffffffull) return fail(ZEN_EINVAL, "zen_momentum_lists: too many entries");
+  if (blocks > (uint64_t)kMostThreads / kBlock) return fail(ZEN_EINVAL, "zen_momentum_lists: too many entries");
   if (n == 0) {
     for (int l = 0; l < lists; ++l)
       if (lengths[l] > 0) return fail(ZEN_EINVAL, "zen_momentum_lists: entries for no elements");

@@ -60,7 +60,7 @@ int pack_matrices(const PackArgs *args, int count, hipStream_t stream) {
     two.blocks[i] = (uint32_t)(across * down * args[i].batch);
     all += two.blocks[i];
   }
-  if (all > 0x7fffffffll) return fail(ZEN_EINVAL, "matrix product: too many rows");
+  if (all > kMostThreads / 256) return fail(ZEN_EINVAL, "matrix product: too many rows");
   k_pack<<<dim3((unsigned)all), dim3(256), 0, stream>>>(two);
   ZEN_LAUNCH_CHECK("k_pack");
   return ZEN_OK;

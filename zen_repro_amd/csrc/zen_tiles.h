@@ -33,6 +33,7 @@ typedef float float16v __attribute__((ext_vector_type(16)));
 constexpr int kTileK = 64;
 constexpr int64_t kMostLd = 1 << 21;  // a step's addresses, 256 rows at most, stay below 2^30
 constexpr int kMostList = 32;  // matrices of separate addresses to a launch
+constexpr int64_t kMostThreads = 0xffffffffll;  // of a launch: the runtime counts them in 32 bits
 
 struct MatOperand {
   const uint16_t *p[2];  // the matrix, and what its rounding to 16 bits left over (itself where there is nothing: never null)
@@ -744,7 +745,8 @@ inline int launch_tiles(MatSize size, const MatOperand &a, const MatOperand &b, 
   size.tiles_m = (size.m + S::BM - 1) / S::BM;
   size.tiles_n = (size.n + S::BN - 1) / S::BN;
   const int64_t tiles = (SYM ? (int64_t)size.tiles_m * (size.tiles_m + 1) / 2 : (int64_t)size.tiles_m * size.tiles_n) * size.batch;
-  if (tiles * (size.splits > S::W * S::FM ? size.splits : S::W * S::FM) > 0x7fffffffll) return fail(ZEN_EINVAL, "matrix product: too many tiles");
+  const int64_t joined = size.splits > 1 ? S::W * S::FM * 64 : 0;
+  if (tiles > kMostThreads / (size.splits * S::threads + joined)) return fail(ZEN_EINVAL, "matrix product: too many tiles");
   k_tiles<S, AK, BK, BF, SYM, Epilogue><<<dim3((unsigned)(tiles * size.splits)), dim3(S::threads), 0, stream>>>(size, a, b, e);
   ZEN_LAUNCH_CHECK("k_tiles");
   if (size.splits > 1) {
