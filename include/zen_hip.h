@@ -753,6 +753,8 @@ int zen_product(const zen_product_args *args);
  * held in 22 bits (two of fp16) and a product is three (results to fp32's accuracy); else the operands of the
  * products are fp16 and X is carried from step to step in 22 bits: results are off by less than bf16 rounds where the smaller side
  * is at least 64, by up to three times that for very small matrices.
+ * The first step's X has singular values up to 1.  Refused are coefficients that can take one, its square (an entry of A) or
+ * b A + c A A (in the last two steps + a - 1) beyond 32752 in any step.
  * rows and cols are at most 2^21.  An update of zeros gives zeros.  outs may be the updates themselves (same type and strides), else nothing overlaps.
  */
 typedef struct zen_orthogonal_args {

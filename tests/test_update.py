@@ -941,3 +941,30 @@ def test_more_threads_than_a_launch_takes_are_refused(L):
     # (k x n, every second element: laid out first)
     assert L.zen_product(product_args(m=64, n=1 << 30, k=1 << 13, b_rs=2, b_cs=1 << 14, out_rs=1 << 30, workspace=256,
                                       workspace_bytes=1 << 62)) == _lib.EINVAL
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("abc,steps", [((70.0, 0.0, 0.0), 1), ((70.0, 0.0, 0.0), 2), ((150.0, 0.0, 0.0), 2), ((8.28, -23.6, 17.3), 2),
+                                       ((3.0, -4.0, 2.0), 5), ((1.0, 0.0, 0.0), 3), ((2.0, 0.0, 0.0), 6), ((0.0, 100.0, 0.0), 1),
+                                       ((-3.4445, 4.7750, -2.0315), 5)])
+@pytest.mark.parametrize("m,n", [(64, 96), (40, 30)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_orthogonalize_with_coefficients_that_take_values_far(abc, steps, m, n, dtype):
+    u = update_like(m, n, 430).to(dtype)
+    want, room = room_of(u, BF16 if dtype == BF16 else F16, steps=steps, abc=abc)
+    got = zen.orthogonalize(u, steps=steps, coefficients=abc)
+    assert got.isfinite().all() and off(got, want) <= room
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("abc,steps", [((8.28, -23.6, 17.3), 5), ((20.0, -100.0, 90.0), 2), ((3.0, -4.0, 2.0), 6), ((4e4, 0.0, 0.0), 1),
+                                       ((200.0, 0.0, 0.0), 3), ((math.nan, 0.0, 0.0), 1), ((1.0, math.inf, 0.0), 1),
+                                       ((1.0, 0.0, -math.inf), 5), ((math.inf, 0.0, 0.0), 5)])
+def test_coefficients_that_would_leave_the_range_are_refused(abc, steps):
+    u = update_like(64, 48, 431)
+    w = u.clone()
+    with pytest.raises(ValueError, match="coefficients"):
+        zen.orthogonalize(u, steps=steps, coefficients=abc)
+    with pytest.raises(ValueError, match="coefficients"):
+        zen.orthogonal_step(w, u, 0.1, steps=steps, coefficients=abc)
+    assert torch.equal(w, u)

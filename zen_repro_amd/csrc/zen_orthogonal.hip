@@ -6,9 +6,9 @@
 // with a transposing read, for 7 us of writing).
 // Bound by the matrix instructions: 3 m m n + m m m flops a step.
 //
-// Everything is held as fp16 times kUnit, with kUnit = 2^10: a value of 1 is far from fp16's limits and what rounding leaves over
-// is far from its denormals.  Why fp16 and not bf16: entries stay below 2, so range is not needed, and the iteration
-// amplifies rounding (errors against 64 bits, Gaussian update 1024 x 1024: bf16 2e-2, fp16 1e-3).  Where a direction starts
+// Everything is held as fp16 times a unit of 2^10: a value of 1 is far from fp16's limits and what rounding leaves over
+// is far from its denormals (coefficients that can take values beyond 63 get smaller units, see Units).  Why fp16 and not
+// bf16: entries stay below 2 or so, range is not needed, and the iteration amplifies rounding (errors against 64 bits, Gaussian update 1024 x 1024: bf16 2e-2, fp16 1e-3).  Where a direction starts
 // small it grows by `a` a step, and so does the noise that rounding X adds to it; so X is carried on as two fp16 (22 bits) and
 // only the products see 11 of them.  The last two steps are written as X + (b A + c A A + (a - 1) I) X: there
 // the singular values are near 1, the bracket is near zero, and so is what rounding it does.  The diagonals of A and of
@@ -16,12 +16,14 @@
 // rows on (64 x 64 to 1024 x 4096; a single strong direction does best, a square Gaussian update worst, and the more rows
 // the better), which is less than rounding it to bf16 does, 1.66e-3.  With `precise`
 // (results of fp32 and fp16) the products see 22 bits of every operand too: A B + A B' + A' B, what is left out is below 2^-22.
+#include <cmath>
+
 #include "zen_tiles.h"
 
 namespace zen {
 namespace {
 
-constexpr float kUnit = 1024.f;
+constexpr double kUnit = 1024.0, kMostHalf = 65504.0;
 constexpr int kSquareBlock = 256;
 constexpr int kMostShares = 1024;  // workgroups to a matrix' sum of squares
 
@@ -101,7 +103,7 @@ __global__ __launch_bounds__(256) void k_lay_out(LayOut p) {
   if ((tid & 63) == 0) s_sum[tid >> 6] = sum;
   __syncthreads();
   const double norm = sqrt((s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3])) + p.eps;
-  const double scale = norm == 0.0 ? 0.0 : (double)kUnit / norm;  // nothing but zeros, and eps is zero
+  const double scale = norm == 0.0 ? 0.0 : kUnit / norm;  // nothing but zeros, and eps is zero
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     const int s = q * 32 + tid / 8, f = tid % 8 * 8;
@@ -137,6 +139,55 @@ struct Room {
   TilePlan gram, square, apply;
   size_t bytes;
 };
+
+// What a step's matrices are held times, powers of two: an entry is at most its matrix' largest singular value, X's begin at
+// one at most, and a step takes an s from [0, top] to p(s) = s (a + b s^2 + c s^4) and X X^T's s^2 to the bracket's value.
+struct Units {
+  double x, a, b;  // of X before the step, A and the bracket
+};
+
+double unit_of(double most) {
+  double unit = kUnit;
+  while (unit * most > kMostHalf * 0.98) unit *= 0.5;  // (roundings on the way are far less than a fiftieth)
+  return unit;
+}
+
+// The largest |f| on [0, end], from its values at both ends and at the roots of its derivative r0 + r1 y + r2 y^2 in between.
+template <class F>
+double most_of(F f, double end, double r0, double r1, double r2) {
+  double most = fmax(fabs(f(0.0)), fabs(f(end)));
+  const auto look = [&](double y) {
+    if (y > 0 && y < end) most = fmax(most, fabs(f(y)));
+  };
+  if (r2 == 0.0) {
+    if (r1 != 0.0) look(-r0 / r1);
+  } else if (const double d = r1 * r1 - 4 * r2 * r0; d >= 0) {
+    const double q = -0.5 * (r1 + copysign(sqrt(d), r1));  // no cancellation
+    look(q / r2);
+    if (q != 0.0) look(r0 / q);
+  }
+  return most;
+}
+
+// Of the step that begins with singular values up to `top`, which becomes the next one's.  Without an answer where a unit would be below
+// one (coefficients that are not finite among them): values around one would come too near to fp16's denormals.
+bool units_of(double a, double b, double c, bool near, double &top, Units &u) {
+  const double end = top * top;
+  const double shift = near ? a - 1.0 : 0.0;
+  const double bracket = most_of([&](double y) { return shift + y * (b + c * y); }, end, b, 2 * c, 0.0);
+  if (!(top < kMostHalf / 2 && end < kMostHalf / 2 && bracket < kMostHalf / 2 && std::isfinite(a))) return false;
+  u = {unit_of(top), unit_of(end), unit_of(bracket)};
+  top = most_of([&](double y) { return sqrt(y) * (a + y * (b + c * y)); }, end, a, 3 * b, 5 * c);
+  return true;
+}
+
+bool holds(const zen_orthogonal_args &p) {
+  double top = 1.0;
+  Units u;
+  for (int step = 0; step < p.steps; ++step)
+    if (!units_of(p.a, p.b, p.c, step >= p.steps - 2, top, u)) return false;
+  return true;
+}
 
 int shares_of(int64_t rows, int64_t cols) {
   const int64_t want = rows * cols / 4096 + 1;
@@ -228,14 +279,19 @@ int chunk(const zen_orthogonal_args &p, const Room &r, int64_t first, int batch,
   const int64_t mm = r.m * r.m, mn = r.m * r.n;
   const MatSize gram = {m, m, n, 0, 0, batch, parts, 1, nullptr}, square = {m, m, m, 0, 0, batch, parts, 1, nullptr},
                 apply = {m, n, m, 0, 0, batch, parts, 1, nullptr};
+  double top = 1.0;
+  Units u, next;
+  units_of(p.a, p.b, p.c, p.steps <= 2, top, next);
   for (int step = 0; step < p.steps; ++step) {
     const int at = step & 1;
     const bool near = step >= p.steps - 2;
+    u = next;
+    if (step + 1 < p.steps) units_of(p.a, p.b, p.c, step + 1 >= p.steps - 2, top, next);
     const MatOperand x = operand(r.x, HALVES ? r.x_low : nullptr, r.n, mn);
     const MatOperand xt = operand(r.turned[at], r.turned_low[at], r.m, mn);
     const MatOperand a = operand(r.a, r.a_low, r.m, mm), b = operand(r.b, r.b_low, r.m, mm);
     KeepEpilogue<kGram, HALVES> g = {};
-    g.alpha = 1.f / kUnit;
+    g.alpha = (float)(u.a / (u.x * u.x));
     g.rows = g.cols = m;
     g.d = r.a;
     g.d_low = r.a_low;
@@ -245,10 +301,10 @@ int chunk(const zen_orthogonal_args &p, const Room &r, int64_t first, int batch,
     g.low_batch = r.m;
     if (const int rc = run_tiles<true, true, false, true>(r.gram, r.partial, gram, x, x, g, s)) return rc;
     KeepEpilogue<kSquare, HALVES> q = {};
-    q.alpha = p.c / kUnit;
-    q.beta = p.b;
+    q.alpha = (float)(p.c * (u.b / (u.a * u.a)));
+    q.beta = (float)(p.b * (u.b / u.a));
     q.rows = q.cols = m;
-    q.diag = near ? (p.a - 1.f) * kUnit : 0.f;
+    q.diag = near ? (float)((p.a - 1.f) * u.b) : 0.f;
     q.diag_n = small;
     q.c = r.a;
     q.c_low = r.a_low;
@@ -262,8 +318,8 @@ int chunk(const zen_orthogonal_args &p, const Room &r, int64_t first, int batch,
     if (const int rc = run_tiles<true, true, false, true>(r.square, r.partial, square, a, a, q, s)) return rc;
     if (step + 1 < p.steps) {
       KeepEpilogue<kApply, HALVES> e = {};
-      e.alpha = 1.f / kUnit;
-      e.beta = near ? 1.f : p.a;
+      e.alpha = (float)(next.x / (u.b * u.x));
+      e.beta = (float)((near ? 1.f : p.a) * (next.x / u.x));
       e.rows = m;
       e.cols = n;
       e.c = e.d = r.x;
@@ -279,8 +335,8 @@ int chunk(const zen_orthogonal_args &p, const Room &r, int64_t first, int batch,
       continue;
     }
     OutEpilogue o = {};
-    o.alpha = 1.f / (kUnit * kUnit);
-    o.beta = (near ? 1.f : p.a) / kUnit;
+    o.alpha = (float)(1.0 / (u.b * u.x));
+    o.beta = (float)((near ? 1.f : p.a) / u.x);
     o.gain = p.weights ? -p.gain : 1.f;
     o.keep = p.keep;
     o.x = r.x;
@@ -340,6 +396,7 @@ int zen_orthogonal(const zen_orthogonal_args *p) {
     if (!p->updates[i] || !p->outs[i]) return fail(ZEN_EINVAL, "zen_orthogonal: null pointer");
   const Room r = room_for(p->rows, p->cols, p->count, p->precise != 0, p->workspace);
   if (p->workspace_bytes < r.bytes) return fail(ZEN_EWORKSPACE, "zen_orthogonal: workspace too small");
+  if (!holds(*p)) return fail(ZEN_EINVAL, "zen_orthogonal: in so many steps these coefficients can take values beyond fp16's range");
   for (int64_t first = 0; first < p->count; first += r.batch) {
     const int64_t rest = p->count - first;
     const int batch = (int)(rest < r.batch ? rest : r.batch);

@@ -136,6 +136,8 @@ def orthogonalize(update, steps=5, coefficients=COEFFICIENTS, eps=1e-7, dtype=No
 
     update  a matrix, a stack (3-D) or a list of matrices of one shape; fp32, bf16 or fp16, any strides, rows and columns
             up to 2^21.  Many small matrices are quicker in one call than one by one
+    coefficients   a, b, c.  A ValueError, if in so many steps they can take a singular value between 0 and 1 (or its square,
+            or b A + c A A) beyond 32752: they would not settle around one
     dtype   the result's type (default: the update's).  It decides the precision: for bf16 the products' operands are
             fp16 where the smaller side is at least 64 (off by less than the result's own rounding then), below
             that, and for fp32 and fp16, they have 22 bits (three products of fp16 each); the iterate has 22 bits
