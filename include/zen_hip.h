@@ -60,8 +60,9 @@ extern "C" {
  *    library
  * 11: such a dictionary's chunk words have 32 bits: built anew
  * 12: ZEN_F16, zen_momentum, zen_momentum_lists, zen_product, zen_orthogonal
+ * 13: zen_product_path, zen_orthogonal_path
  */
-#define ZEN_ABI_VERSION 12
+#define ZEN_ABI_VERSION 13
 
 #define ZEN_F32 0
 #define ZEN_BF16 1
@@ -744,6 +745,10 @@ typedef struct zen_product_args {
 } zen_product_args;
 size_t zen_product_workspace(const zen_product_args *args); /* 0: none is needed */
 int zen_product(const zen_product_args *args);
+/* What the call takes: the tile's side (bits 0 to 9), workgroups to a compute unit (10, 11), workgroups that share a tile's steps
+   (12 to 19), whether a (20) and b (21) are read with k as the stride, and whether a (22) and b (23) are laid out first; negative:
+   bad arguments.  Results differ in the order of sums at most. */
+int zen_product_path(const zen_product_args *args);
 
 /*
  * Orthogonalisation of updates (rows x cols, `count` of them, one type and one pair of strides) by Newton-Schulz steps:
@@ -777,6 +782,8 @@ typedef struct zen_orthogonal_args {
 } zen_orthogonal_args;
 size_t zen_orthogonal_workspace(int64_t rows, int64_t cols, int64_t count, int precise);
 int zen_orthogonal(const zen_orthogonal_args *args);
+/* The same bits of a step's products: 0: X X^T, 1: A A, 2: the bracket and X. */
+int zen_orthogonal_path(int64_t rows, int64_t cols, int64_t count, int precise, int product);
 
 #ifdef __cplusplus
 }

@@ -42,7 +42,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("ZEN_HIP_LIB") or os.path.join(_HERE, "csrc", "libzen_hip.so")
 
 # ZEN_ABI_VERSION of include/zen_hip.h this loader's signatures and structs are written for
-ABI_VERSION = 12
+ABI_VERSION = 13
 MOMENTUM_LISTS_MOST = 64  # ZEN_MOMENTUM_LISTS_MOST
 TABLE_SIZES_MOST = 1024  # ZEN_TABLE_SIZES_MOST
 
@@ -186,8 +186,10 @@ def lib():
         "zen_momentum_lists": (i32, [vp, i32, vp, i32, vp, i32, vp, vp, i32, i64, ctypes.c_float, i32, vp, i32, vp, sz, vp, vp]),
         "zen_product_workspace": (sz, [vp]),
         "zen_product": (i32, [vp]),
+        "zen_product_path": (i32, [vp]),
         "zen_orthogonal_workspace": (sz, [i64, i64, i64, i32]),
         "zen_orthogonal": (i32, [vp]),
+        "zen_orthogonal_path": (i32, [i64, i64, i64, i32, i32]),
         "zen_stream_read": (i32, [vp, sz, vp, vp]),
         "zen_profile_enable": (i32, [i32]),
         "zen_profile_only": (i32, [i32]),

@@ -380,6 +380,14 @@ size_t zen_orthogonal_workspace(int64_t rows, int64_t cols, int64_t count, int p
   return room_for(rows, cols, count, precise != 0, nullptr).bytes;
 }
 
+int zen_orthogonal_path(int64_t rows, int64_t cols, int64_t count, int precise, int product) {
+  using namespace zen;
+  if (rows <= 0 || cols <= 0 || count <= 0 || rows > kMostSide || cols > kMostSide || product < 0 || product > 2)
+    return fail(ZEN_EINVAL, "zen_orthogonal_path: a size is out of range");
+  const Room r = room_for(rows, cols, count, precise != 0, nullptr);
+  return path_of(product == 0 ? r.gram : product == 1 ? r.square : r.apply);
+}
+
 int zen_orthogonal(const zen_orthogonal_args *p) {
   using namespace zen;
   if (!p) return fail(ZEN_EINVAL, "zen_orthogonal: null pointer");

@@ -106,6 +106,14 @@ size_t zen_product_workspace(const zen_product_args *p) {
   return room(a, p->batch) + room(b, p->batch) + plan(*p, a, b).partial_bytes;
 }
 
+int zen_product_path(const zen_product_args *p) {
+  using namespace zen;
+  if (const int rc = check(p)) return rc;
+  const Side a = side_a(*p), b = side_b(*p);
+  return path_of(plan(*p, a, b)) | (a.contiguous ? 0 : 1 << 20) | (b.contiguous ? 0 : 1 << 21) | (a.packed ? 1 << 22 : 0) |
+         (b.packed ? 1 << 23 : 0);
+}
+
 int zen_product(const zen_product_args *p) {
   using namespace zen;
   if (const int rc = check(p)) return rc;

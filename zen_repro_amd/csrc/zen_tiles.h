@@ -780,6 +780,9 @@ struct TilePlan {
   size_t partial_bytes;
 };
 
+// What the *_path calls say of it (include/zen_hip.h).
+inline int path_of(const TilePlan &p) { return p.side | p.at_once << 10 | p.splits << 12; }
+
 inline TilePlan plan_tiles(int64_t m, int64_t n, int64_t k, int parts, int64_t batch, bool sym, bool by_k) {
   const int64_t steps = ceil_div(k, kTileK) * parts;
   TilePlan best = {64, 2, 1, 0};
