@@ -121,6 +121,25 @@ def test_product_on_every_tile(m, n, k, a_strided, b_strided, symmetric, name, s
         assert room.eq(7.0).all()
 
 
+def among_nans(rows, cols, seed, dtype):
+    """A matrix with NaN behind it, whole tiles and steps far, in rows and in columns."""
+    room = torch.full((rows + 512, up8(cols) + 512), float("nan"), device="cuda", dtype=dtype)
+    room[:rows, :cols] = normal((rows, cols), seed, dtype)
+    return room[:rows, :cols]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rest", [8, 40])  # k in the last step; the loads behind its first one begin in the middle of it and behind it
+@pytest.mark.parametrize("m,n,k,a_strided,b_strided,symmetric,name,split", [p for p in PRODUCTS if not p[5]])
+def test_nothing_behind_an_operand_comes_in(m, n, k, a_strided, b_strided, symmetric, name, split, rest):
+    k += rest - k % 64
+    a = among_nans(k, m, 530, F16).t() if a_strided else among_nans(m, k, 530, F16)
+    b = among_nans(k, n, 531, F16) if b_strided else among_nans(n, k, 531, F16).t()
+    tiled = product_tile(m, n, k, (*a.stride(), 0), (*b.stride(), 0))
+    assert tiled == (name, split, a_strided, b_strided)
+    product_check(zen.product(a, b), a, b, None, 1.0, 0.0)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("count,m,n,k,name", STACKS)
 def test_product_of_stacks_on_large_tiles(count, m, n, k, name):
