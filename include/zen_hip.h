@@ -780,6 +780,7 @@ typedef struct zen_orthogonal_args {
   size_t workspace_bytes;
   void *stream;
 } zen_orthogonal_args;
+/* Many matrices take turns in some 2 GiB; one by itself takes what it takes: 12 bytes an element of a square one, 20 with `precise`. */
 size_t zen_orthogonal_workspace(int64_t rows, int64_t cols, int64_t count, int precise);
 int zen_orthogonal(const zen_orthogonal_args *args);
 /* The same bits of a step's products: 0: X X^T, 1: A A, 2: the bracket and X. */

@@ -968,3 +968,13 @@ def test_coefficients_that_would_leave_the_range_are_refused(abc, steps):
     with pytest.raises(ValueError, match="coefficients"):
         zen.orthogonal_step(w, u, 0.1, steps=steps, coefficients=abc)
     assert torch.equal(w, u)
+
+
+@pytest.mark.parametrize("m,n", [(4096, 4096), (2048, 2048), (4096, 1024), (1000, 30000), (8192, 4096)])
+@pytest.mark.parametrize("precise", [0, 1])
+def test_a_stacks_workspace_stays_near_two_gib(L, m, n, precise):
+    """Whatever its length: 2 GiB, beside sums of split tiles (512 tiles of 256 x 256 in fp32) and of squares (8 KiB a matrix)."""
+    for count in (1, 7, 40, 1000):
+        assert L.zen_orthogonal_workspace(m, n, count, precise) <= (2 << 30) + 512 * 256 * 256 * 4 + (1 << 20)
+    few = L.zen_orthogonal_workspace(m, n, 40, precise)
+    assert L.zen_orthogonal_workspace(m, n, 1000, precise) == few > L.zen_orthogonal_workspace(m, n, 1, precise)

@@ -194,9 +194,10 @@ int shares_of(int64_t rows, int64_t cols) {
   return (int)(want < kMostShares ? want : kMostShares);
 }
 
-int chunk_of(int64_t m, int64_t n, int64_t count) {
-  // enough matrices at once to fill the card, no more room than some 2 GiB where one matrix does
-  int64_t most = (1ll << 28) / (m * n);
+int chunk_of(int64_t m, int64_t n, int64_t count, bool precise) {
+  // enough matrices at once to fill the card, in no more room than 2 GiB (and the split sums') where one matrix does
+  const int64_t bytes = 2 * (precise ? 6 * m * n + 4 * m * m : 4 * m * n + 2 * m * m);
+  int64_t most = (1ll << 31) / bytes;
   if (most < 1) most = 1;
   if (most > kMostList) most = kMostList;
   return (int)(count < most ? count : most);
@@ -207,7 +208,7 @@ Room room_for(int64_t rows, int64_t cols, int64_t count, bool precise, void *at)
   const int64_t small = rows < cols ? rows : cols, large = rows < cols ? cols : rows;
   r.m = ceil_div(small, kTileK) * kTileK;
   r.n = ceil_div(large, kTileK) * kTileK;
-  r.batch = chunk_of(r.m, r.n, count);
+  r.batch = chunk_of(r.m, r.n, count, precise);
   Carver cv(at);
   const size_t xs = (size_t)r.batch * r.m * r.n, as = (size_t)r.batch * r.m * r.m;
   r.x = cv.take<_Float16>(xs);
