@@ -755,7 +755,7 @@ int zen_product_path(const zen_product_args *args);
  *   X = U / (|U|_F + eps);   `steps` times  X = a X + (b A + c A A) X  with A = X X^T (X with rows <= cols: turned if need be)
  * and out = X (weights null), or, applied to weights in place,  W = keep * W - gain * X.
  * updates, outs and weights are HOST arrays of device addresses.  Types: any of the three for each.  `precise`: every operand is
- * held in 22 bits (two of fp16) and a product is three (results to fp32's accuracy); else the operands of the
+ * held in 22 bits (two of fp16) and a product is three (off by up to twice what fp32 products are); else the operands of the
  * products are fp16 and X is carried from step to step in 22 bits: results are off by less than bf16 rounds where the smaller side
  * is at least 64, by up to three times that for very small matrices.
  * The first step's X has singular values up to 1.  Refused are coefficients that can take one, its square (an entry of A) or

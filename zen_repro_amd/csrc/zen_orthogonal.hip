@@ -15,7 +15,8 @@
 // the bracket are kept whole (KeepEpilogue).  Before its own rounding a result is then off by 0.24 to 1.24e-3 from 64
 // rows on (64 x 64 to 1024 x 4096; a single strong direction does best, a square Gaussian update worst, and the more rows
 // the better), which is less than rounding it to bf16 does, 1.66e-3.  With `precise`
-// (results of fp32 and fp16) the products see 22 bits of every operand too: A B + A B' + A' B, what is left out is below 2^-22.
+// (results of fp32 and fp16) the products see 22 bits of every operand too: A B + A B' + A' B, what is left out is below 2^-22; off
+// by half to twice what products in fp32 are (twice: one strong direction, whose fellows grow out of X's 22 bits).
 #include <cmath>
 
 #include "zen_tiles.h"

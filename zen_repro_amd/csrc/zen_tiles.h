@@ -9,7 +9,7 @@
 // transposed in memory.  The range check of the buffer loads puts zeros where the tile hangs over the operand's end.
 //
 // What bounds it: with 256 x 256 tiles a step's products take a compute unit 2048 cycles, of some 2900 (8192^3, k contiguous:
-// matrix cores busy 71 % of the cycles, LDS 20 %, and a clock that the power limit holds at 1.5 to 1.9 GHz: 1110 to 1260
+// matrix cores busy 71 % of the cycles, LDS 20 %, and a clock that the power limit holds at 1.5 to 1.9 GHz: 1200 to 1310
 // TFLOP/s; without the loads, 1550).  What mattered most: reads, loads and products in an order of our own, one by one (the
 // compiler's: 1.79 against 1.50 million cycles at that size), and reads of LDS without bank conflicts.
 //

@@ -80,12 +80,14 @@ def momentum_update_sparse(momentum, indices_tensors, values_tensors, mu=0.95, n
 
 
 def product(a, b, residual=None, alpha=1.0, beta=1.0, symmetric=False, dtype=None, out=None):
-    """alpha * a @ b + beta * residual, summed in fp32 and rounded once.
+    """alpha * a @ b + beta * residual, summed in fp32 and rounded once.  torch.addmm is up to a fifth quicker on large
+    matrices of one type; this also takes results and residuals of other types, symmetric results and any strides.
 
     a, b       bf16 or fp16 matrices (m x k and k x n), or stacks of as many; any strides.  Where rows or columns are contiguous
                and begin at multiples of 16 bytes they are read as they lie (a transposed view costs nothing), else
                laid out first.  k is at most 2^21, a stack of 65535 matrices
-    residual   m x n (or a stack), fp32, bf16 or fp16, any strides.  It is read whatever beta is: NaN in it stays NaN
+    residual   m x n (or a stack), fp32, bf16 or fp16, any strides (quickest where it lies as the result does).  It is read
+               whatever beta is: NaN in it stays NaN
     symmetric  the caller vouches that a @ b is symmetric (a matrix and its own transpose, powers of a symmetric
                matrix): half of it is computed and mirrored
     dtype      the result's type (default: the residual's, else a's): fp32, bf16 or fp16
@@ -140,7 +142,8 @@ def orthogonalize(update, steps=5, coefficients=COEFFICIENTS, eps=1e-7, dtype=No
             or b A + c A A) beyond 32752: they would not settle around one
     dtype   the result's type (default: the update's).  It decides the precision: for bf16 the products' operands are
             fp16 where the smaller side is at least 64 (off by less than the result's own rounding then), below
-            that, and for fp32 and fp16, they have 22 bits (three products of fp16 each); the iterate has 22 bits
+            that, and for fp32 and fp16, they have 22 bits (three products of fp16 each, off by up to twice what products in
+            fp32 are); the iterate has 22 bits
     out     where the result goes, of the update's shape (a list for a list); may be the update itself"""
     updates = _matrices(update, "update")
     listed = isinstance(update, (list, tuple))
