@@ -760,7 +760,8 @@ int zen_product_path(const zen_product_args *args);
  * is at least 64, by up to three times that for very small matrices.
  * The first step's X has singular values up to 1.  Refused are coefficients that can take one, its square (an entry of A) or
  * b A + c A A (in the last two steps + a - 1) beyond 32752 in any step.
- * rows and cols are at most 2^21.  An update of zeros gives zeros.  outs may be the updates themselves (same type and strides), else nothing overlaps.
+ * rows and cols are at most 2^21.  An update of zeros gives zeros.  outs may be the updates themselves (same type and
+ * strides), else nothing overlaps.
  */
 typedef struct zen_orthogonal_args {
   const void *const *updates;

@@ -435,7 +435,8 @@ py::tuple momentum(const py::object &fn, const Tensor &momentum, const Tensor &g
   return py::make_tuple(rc, out);
 }
 
-// counts: none, one tensor (an element to a list), or one tensor or none to a list; before: the status word of the call that made the lists
+// counts: none, one tensor (an element to a list), or one tensor or none to a list
+// before: the status word of the call that made the lists
 py::tuple momentum_lists(const py::object &fn, Zeros &zeros, const Tensor &momentum, const std::vector<Tensor> &indices,
                          const std::vector<Tensor> &values, double mu, bool nesterov, const std::optional<Tensor> &counted,
                          const std::optional<std::vector<std::optional<Tensor>>> &counts, const Dtype &dtype,

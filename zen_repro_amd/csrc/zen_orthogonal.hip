@@ -6,17 +6,18 @@
 // with a transposing read, for 7 us of writing).
 // Bound by the matrix instructions: 3 m m n + m m m flops a step.
 //
-// Everything is held as fp16 times a unit of 2^10: a value of 1 is far from fp16's limits and what rounding leaves over
-// is far from its denormals (coefficients that can take values beyond 63 get smaller units, see Units).  Why fp16 and not
-// bf16: entries stay below 2 or so, range is not needed, and the iteration amplifies rounding (errors against 64 bits, Gaussian update 1024 x 1024: bf16 2e-2, fp16 1e-3).  Where a direction starts
-// small it grows by `a` a step, and so does the noise that rounding X adds to it; so X is carried on as two fp16 (22 bits) and
-// only the products see 11 of them.  The last two steps are written as X + (b A + c A A + (a - 1) I) X: there
-// the singular values are near 1, the bracket is near zero, and so is what rounding it does.  The diagonals of A and of
-// the bracket are kept whole (KeepEpilogue).  Before its own rounding a result is then off by 0.24 to 1.24e-3 from 64
-// rows on (64 x 64 to 1024 x 4096; a single strong direction does best, a square Gaussian update worst, and the more rows
-// the better), which is less than rounding it to bf16 does, 1.66e-3.  With `precise`
-// (results of fp32 and fp16) the products see 22 bits of every operand too: A B + A B' + A' B, what is left out is below 2^-22; off
-// by half to twice what products in fp32 are (twice: one strong direction, whose fellows grow out of X's 22 bits).
+// Everything is held as fp16 times a unit of 2^10: a value of 1 is far from fp16's limits and what rounding leaves over is far
+// from its denormals (coefficients that can take values beyond 63 get smaller units, see Units).  Why fp16 and not bf16:
+// entries stay below 2 or so, range is not needed, and the iteration amplifies rounding (errors against 64 bits, Gaussian
+// update 1024 x 1024: bf16 2e-2, fp16 1e-3).  Where a direction starts small it grows by `a` a step, and so does the noise
+// that rounding X adds to it; so X is carried on as two fp16 (22 bits) and only the products see 11 of them.  The last two
+// steps are written as X + (b A + c A A + (a - 1) I) X: there the singular values are near 1, the bracket is near zero, and
+// so is what rounding it does.  The diagonals of A and of the bracket are kept whole (KeepEpilogue).  Before its own
+// rounding a result is then off by 0.24 to 1.24e-3 from 64 rows on (64 x 64 to 1024 x 4096; a single strong direction does
+// best, a square Gaussian update worst, and the more rows the better), which is less than rounding it to bf16 does, 1.66e-3.
+// With `precise` (results of fp32 and fp16) the products see 22 bits of every operand too: A B + A B' + A' B, what is left
+// out is below 2^-22; off by half to twice what products in fp32 are (twice: one strong direction, whose fellows grow out
+// of X's 22 bits).
 #include <cmath>
 
 #include "zen_tiles.h"
